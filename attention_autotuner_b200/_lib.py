@@ -6,12 +6,13 @@ import ctypes
 import os
 import threading
 
-from .build import LIB_PATH
+from .build import KV_PATH, LIB_PATH
 
 F16, BF16 = 0, 1
 
 _lock = threading.Lock()
 _lib = None
+_kv = None
 
 
 class AttnB200Error(RuntimeError):
@@ -101,3 +102,48 @@ def check(code: int):
 
 def device_status(clear: bool = True) -> int:
     return load().attn_b200_device_status(1 if clear else 0)
+
+
+class KVCacheStruct(ctypes.Structure):
+    """attn_b200_kv_cache (include/attn_b200_kv.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("num_pages", ctypes.c_int), ("heads", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("bits", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+def _declare_kv(lib):
+    vp, ci, cs = ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(KVCacheStruct)
+    strides = ctypes.POINTER(ctypes.c_longlong)
+    lib.attn_b200_kv_last_error.restype = ctypes.c_char_p
+    lib.attn_b200_kv_last_error.argtypes = []
+    for name, res, args in (
+            ("status", ci, [ci]), ("prepare", ci, []), ("block_bytes", ci, [ci, ci]),
+            ("write", ci, [cs, vp, ci, ci, vp, vp, vp, strides, vp, strides, ci, ci, vp]),
+            ("read", ci, [cs, vp, ci, ci, vp, vp, vp, vp, ci, ci, vp]),
+            ("attn_workspace_bytes", ctypes.c_size_t, [cs, ci, ci, ci]),
+            ("attn", ci, [vp, cs, vp, ci, ci, vp, vp, vp, vp, ctypes.c_size_t, ci, ci, ci, ctypes.c_float, ci, vp])):
+        fn = getattr(lib, "attn_b200_kv_" + name)
+        fn.restype, fn.argtypes = res, args
+
+
+def load_kv():
+    """libattn_b200_kv.so; raises if it has not been built (python -m attention_autotuner_b200.build)."""
+    global _kv
+    with _lock:
+        if _kv is None:
+            if not os.path.exists(KV_PATH):
+                raise RuntimeError(f"{KV_PATH} is missing: build it with `python -m attention_autotuner_b200.build`. "
+                                   "There is no fallback.")
+            lib = ctypes.CDLL(KV_PATH)
+            _declare_kv(lib)
+            _kv = lib
+    return _kv
+
+
+def check_kv(code: int):
+    if code != 0:
+        raise AttnB200Error(code, load_kv().attn_b200_kv_last_error().decode())
+
+
+def kv_status(clear: bool = True) -> int:
+    """Status word of libattn_b200_kv.so on the current device (attn_b200_kv_status); synchronises."""
+    return load_kv().attn_b200_kv_status(1 if clear else 0)

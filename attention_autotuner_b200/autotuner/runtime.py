@@ -31,12 +31,14 @@ _source_tag_cache = None
 
 def source_tag() -> str:
     """Short hash of the kernel sources; part of every per-config library name, so that libraries built
-    from older sources are never picked up."""
+    from older sources are never picked up. csrc/kv/ is a library of its own that no configuration includes."""
     global _source_tag_cache
     if _source_tag_cache is None:
         import hashlib
         h = hashlib.sha1()
         for root, _dirs, files in sorted(os.walk(CSRC_DIR)):
+            if os.path.basename(root) == "kv":
+                continue
             for name in sorted(files):
                 if name.endswith((".cuh", ".cu", ".h", ".py")):
                     with open(os.path.join(root, name), "rb") as f:

@@ -1,4 +1,5 @@
-"""Builds libattn_b200.so (the C-ABI library of include/attn_b200.h) in-tree with nvcc for sm_100a.
+"""Builds libattn_b200.so (the C-ABI library of include/attn_b200.h) and libattn_b200_kv.so (include/attn_b200_kv.h) in-tree with
+nvcc for sm_100a, and the native operator layer.
 
     python -m attention_autotuner_b200.build [--force] [--benchmarks]
 
@@ -76,6 +77,44 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+# The quantised KV cache (csrc/kv/, include/attn_b200_kv.h): a library of its own.
+KV_DIR = os.path.join(CSRC, "kv")
+KV_PATH = os.path.join(KV_DIR, "libattn_b200_kv.so")
+
+
+def kv_source_hash() -> str:
+    """Hash of what the library is compiled from: csrc/kv/, the headers it takes from csrc/, its C ABI and the flags."""
+    import hashlib
+    h = hashlib.sha1(" ".join(NVCC_FLAGS).encode())
+    paths = [os.path.join(KV_DIR, n) for n in sorted(os.listdir(KV_DIR)) if n.endswith((".cu", ".cuh"))]
+    paths += [os.path.join(CSRC, n) for n in ("fast_div.cuh", "host_common.cuh", "ptx.cuh")]
+    for path in paths + [os.path.join(CSRC, "..", "..", "include", "attn_b200_kv.h")]:
+        with open(path, "rb") as f:
+            h.update(os.path.basename(path).encode() + b"\0" + f.read() + b"\0")
+    return h.hexdigest()
+
+
+def build_kv_library(force: bool = False, verbose: bool = False) -> str:
+    """Compiles csrc/kv/kv_cache.cu into csrc/kv/libattn_b200_kv.so; rebuilt when kv_source_hash changes."""
+    stamp, want = KV_PATH + ".srchash", kv_source_hash()
+    try:
+        with open(stamp) as f:
+            fresh = f.read().strip() == want
+    except OSError:
+        fresh = False
+    if not force and fresh and os.path.exists(KV_PATH):
+        return KV_PATH
+    cmd = [NVCC, *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-o", KV_PATH, os.path.join(KV_DIR, "kv_cache.cu")]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+    if verbose:
+        print(res.stderr)
+    with open(stamp, "w") as f:
+        f.write(want + "\n")
+    return KV_PATH
+
+
 # The native operator layer (csrc/host/torch_ops.cpp): a CPython extension against the installed PyTorch's headers, no
 # CUDA code of its own. It is loaded by ops/_native.py.
 OPS_SRC = os.path.join(CSRC, "host", "torch_ops.cpp")
@@ -91,7 +130,8 @@ def _ops_hash() -> str:
     import hashlib
     import torch
     h = hashlib.sha1(f"{torch.__version__} {sys.version_info[:2]} {OPS_FLAGS} {OPS_LIBS}".encode())
-    for path in (OPS_SRC, os.path.join(CSRC, "..", "..", "include", "attn_b200.h")):
+    include = os.path.join(CSRC, "..", "..", "include")
+    for path in (OPS_SRC, os.path.join(include, "attn_b200.h"), os.path.join(include, "attn_b200_kv.h")):
         with open(path, "rb") as f:
             h.update(f.read())
     return h.hexdigest()
@@ -170,6 +210,7 @@ def build_benchmarks(force: bool = False) -> list:
 
 if __name__ == "__main__":
     print(build_library(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_kv_library(force="--force" in sys.argv, verbose="-v" in sys.argv))
     print(build_torch_ops(force="--force" in sys.argv))
     if "--benchmarks" in sys.argv:
         print("\n".join(build_benchmarks(force="--force" in sys.argv)))

@@ -16,7 +16,7 @@ def install():
         mod = importlib.import_module(f"attention_autotuner_b200.{name}")
         sys.modules.setdefault(name, mod)
     for sub in ("autotuner.runtime", "autotuner.tunner", "autotuner.base_tunner", "autotuner.configs",
-                "ops.attention_interface", "ops.retnet_interface", "utils.ref_op", "utils.misc"):
+                "ops.attention_interface", "ops.cache_interface", "ops.retnet_interface", "utils.ref_op", "utils.misc"):
         try:
             mod = importlib.import_module(f"attention_autotuner_b200.{sub}")
         except ImportError:

@@ -27,6 +27,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include "../../../include/attn_b200_kv.h"
+
+#include <climits>
 #include <cstdlib>
 #include <initializer_list>
 #include <string>
@@ -508,6 +511,178 @@ PyObject* py_chunkwise(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ quantised KV cache
+struct {
+  decltype(&attn_b200_kv_last_error) last_error = nullptr;
+  decltype(&attn_b200_kv_block_bytes) block_bytes = nullptr;
+  decltype(&attn_b200_kv_write) write = nullptr;
+  decltype(&attn_b200_kv_read) read = nullptr;
+  decltype(&attn_b200_kv_attn_workspace_bytes) attn_ws = nullptr;
+  decltype(&attn_b200_kv_attn) attn = nullptr;
+} g_kv;
+
+void check_kv_rc(int rc) {
+  if (rc == 0) return;
+  const std::string text = g_kv.last_error();
+  py::gil_scoped_acquire gil;
+  throw_python(PyObject_CallFunction(g_lib_error, "is", rc, text.c_str()));
+}
+
+// A cache as ops/cache_interface.py keeps it: data [pages, heads, page_size / 16, block bytes], bits, head_dim, dtype (0, 1).
+struct KvCacheArg {
+  Tensor data;
+  attn_b200_kv_cache c{};
+  at::ScalarType dtype = at::kHalf;
+};
+bool take_cache(PyObject* const* a, KvCacheArg& k) {  // data, bits, head_dim, dtype
+  if (!take_tensor(a[0], k.data)) return false;
+  const long bits = PyLong_AsLong(a[1]), d = PyLong_AsLong(a[2]), dt = PyLong_AsLong(a[3]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  const Tensor& t = k.data;
+  if (t.dim() != 4 || t.scalar_type() != at::kByte || !t.is_cuda() || !t.is_contiguous() || t.numel() == 0) return false;
+  if ((bits != 4 && bits != 8) || (d != 64 && d != 128 && d != 256) || t.size(3) != g_kv.block_bytes(bits, d)) return false;
+  if (t.size(0) > INT_MAX || t.size(1) > INT_MAX || t.size(2) > 4096) return false;
+  k.c = {t.data_ptr(), i32(t.size(0)), i32(t.size(1)), i32(t.size(2)) * 16, static_cast<int>(d), static_cast<int>(bits), static_cast<int>(dt)};
+  k.dtype = dt == 0 ? at::kHalf : at::kBFloat16;
+  return true;
+}
+// int32 [B, width] on the cache's device
+bool table_ok(const Tensor& t, const KvCacheArg& k) {
+  return t.dim() == 2 && t.scalar_type() == at::kInt && t.device() == k.data.device() && t.size(0) > 0 && t.size(0) <= INT_MAX &&
+         t.size(1) > 0 && t.size(1) <= INT_MAX;
+}
+bool per_sequence_ok(const Tensor& t, const Tensor& table) {
+  return t.dim() == 1 && t.scalar_type() == at::kInt && t.device() == table.device() && t.size(0) == table.size(0);
+}
+// rows as they are where they are dense and lie apart by what an int holds
+Tensor table_rows(const Tensor& t) {
+  const bool rows = (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || (t.stride(0) >= t.size(1) && t.stride(0) <= INT_MAX));
+  return rows ? t : t.contiguous();
+}
+int table_stride(const Tensor& t) { return i32(t.size(0) == 1 ? t.size(1) : t.stride(0)); }
+bool kv_tensor_ok(const Tensor& t, const KvCacheArg& k) {
+  return t.dim() == 4 && t.scalar_type() == k.dtype && t.device() == k.data.device() && t.size(3) == k.c.head_dim;
+}
+bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
+// k or v as it is if its channels are dense and its rows start at multiples of 16 bytes, else a copy; strides of dimensions of one are 0
+Tensor kv_rows(const Tensor& t, long long* strides) {
+  bool fits = t.stride(3) == 1 && aligned16(t);
+  for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) == 1 || t.stride(i) % 8 == 0);
+  const Tensor r = fits ? t : t.clone(at::MemoryFormat::Contiguous);
+  for (int i = 0; i < 3; ++i) strides[i] = r.size(i) == 1 ? 0 : r.stride(i);
+  return r;
+}
+
+// kv_write(data, bits, head_dim, dtype, table, start, count | None, k, v) -> True | None
+PyObject* py_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 9, "kv_write")) return nullptr;
+  KvCacheArg c;
+  Tensor table, start, count, k, v;
+  if (!take_cache(a, c) || !take_tensor(a[4], table) || !take_tensor(a[5], start) || !take_tensor(a[6], count, true) ||
+      !take_tensor(a[7], k) || !take_tensor(a[8], v) || !table_ok(table, c) || !per_sequence_ok(start, table) ||
+      (count.defined() && !per_sequence_ok(count, table)) || !kv_tensor_ok(k, c) || !kv_tensor_ok(v, c) || k.sizes() != v.sizes() ||
+      k.size(0) != table.size(0) || k.size(1) != c.c.heads || k.size(2) <= 0 || k.size(2) > (1 << 30) || any_grad({&k, &v}))
+    return none();
+  {
+    py::gil_scoped_release nogil;
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(c.data.device());
+    long long ks[3], vs[3];
+    const Tensor kr = kv_rows(k, ks), vr = kv_rows(v, vs), rows = table_rows(table), st = start.contiguous();
+    const Tensor ct = count.defined() ? count.contiguous() : count;
+    check_kv_rc(g_kv.write(&c.c, rows.const_data_ptr<int>(), table_stride(rows), i32(rows.size(1)), st.const_data_ptr<int>(),
+                           static_cast<const int*>(ptr(ct)), ptr(kr), ks, ptr(vr), vs, i32(k.size(0)), i32(k.size(2)), stream_of(c.data)));
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_read(data, bits, head_dim, dtype, table, start | None, count | None, length) -> (k, v) | None
+PyObject* py_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 8, "kv_read")) return nullptr;
+  KvCacheArg c;
+  Tensor table, start, count;
+  if (!take_cache(a, c) || !take_tensor(a[4], table) || !take_tensor(a[5], start, true) || !take_tensor(a[6], count, true) ||
+      !table_ok(table, c) || (start.defined() && !per_sequence_ok(start, table)) || (count.defined() && !per_sequence_ok(count, table)))
+    return none();
+  const long long length = PyLong_AsLongLong(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  if (length <= 0 || length > (1 << 30)) return none();
+  Tensor k, v;
+  {
+    py::gil_scoped_release nogil;
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(c.data.device());
+    const Tensor rows = table_rows(table), st = start.defined() ? start.contiguous() : start, ct = count.defined() ? count.contiguous() : count;
+    k = at::empty({table.size(0), c.c.heads, length, c.c.head_dim}, c.data.options().dtype(c.dtype));
+    v = at::empty_like(k);
+    check_kv_rc(g_kv.read(&c.c, rows.const_data_ptr<int>(), table_stride(rows), i32(rows.size(1)), static_cast<const int*>(ptr(st)),
+                          static_cast<const int*>(ptr(ct)), ptr(k), ptr(v), i32(table.size(0)), i32(length), stream_of(c.data)));
+  }
+  PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
+  return Py_BuildValue("(NN)", pk, pv);
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_attn(data, bits, head_dim, dtype, table, lengths, q, scale, causal, return_lse) -> o | (o, lse) | None
+PyObject* py_kv_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 10, "kv_attn")) return nullptr;
+  KvCacheArg c;
+  Tensor table, lengths, q;
+  if (!take_cache(a, c) || !take_tensor(a[4], table) || !take_tensor(a[5], lengths) || !take_tensor(a[6], q) || !table_ok(table, c) ||
+      !per_sequence_ok(lengths, table) || !kv_tensor_ok(q, c) || q.size(0) != table.size(0) || q.size(1) <= 0 ||
+      q.size(1) % c.c.heads != 0 || q.size(2) <= 0 || q.size(2) > ATTN_B200_KV_MAX_QUERIES || any_grad({&q}))
+    return none();
+  const double scale = PyFloat_AsDouble(a[7]);
+  if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+  const int causal = PyObject_IsTrue(a[8]), ret_lse = PyObject_IsTrue(a[9]);
+  if (causal < 0 || ret_lse < 0) return nullptr;
+  Tensor o, lse;
+  {
+    py::gil_scoped_release nogil;
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(c.data.device());
+    Tensor qc = q.contiguous();
+    if (!aligned16(qc)) qc = qc.clone();
+    const Tensor rows = table_rows(table), len = lengths.contiguous();
+    const int B = i32(q.size(0)), group = i32(q.size(1) / c.c.heads), Lq = i32(q.size(2));
+    o = at::empty(q.sizes(), q.options());
+    if (ret_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    const size_t bytes = g_kv.attn_ws(&c.c, B, group, Lq);
+    Tensor ws;
+    if (bytes != 0) ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    // without a workspace the sizes are not supported: the library says which
+    check_kv_rc(g_kv.attn(ptr(qc), &c.c, rows.const_data_ptr<int>(), table_stride(rows), i32(rows.size(1)), len.const_data_ptr<int>(), ptr(o),
+                          static_cast<float*>(ptr(lse)), bytes != 0 ? ptr(ws) : ptr(o), bytes, B, group, Lq, static_cast<float>(scale),
+                          causal, stream_of(c.data)));
+  }
+  if (!ret_lse) return THPVariable_Wrap(std::move(o));
+  PyObject *po = THPVariable_Wrap(std::move(o)), *pl = THPVariable_Wrap(std::move(lse));
+  return Py_BuildValue("(NN)", po, pl);
+  END_HANDLE_TH_ERRORS
+}
+
+// init_kv(last_error, block_bytes, write, read, attn workspace bytes, attn): addresses in libattn_b200_kv.so
+PyObject* py_init_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 6, "init_kv")) return nullptr;
+  auto addr = [&](int i) { return py::cast<uintptr_t>(py::handle(a[i])); };
+  g_kv.last_error = reinterpret_cast<decltype(g_kv.last_error)>(addr(0));
+  g_kv.block_bytes = reinterpret_cast<decltype(g_kv.block_bytes)>(addr(1));
+  g_kv.write = reinterpret_cast<decltype(g_kv.write)>(addr(2));
+  g_kv.read = reinterpret_cast<decltype(g_kv.read)>(addr(3));
+  g_kv.attn_ws = reinterpret_cast<decltype(g_kv.attn_ws)>(addr(4));
+  g_kv.attn = reinterpret_cast<decltype(g_kv.attn)>(addr(5));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // make_plan(entry point, last_error, library name, [paths], [environment variables]) -> plan, stamped with the files' times
 // and the variables' values of this moment. What the plan is made from is to be read after that: then a change in between
 // makes the plan stale instead of being taken as seen. The entry point may follow with set_entry; a plan without one is
@@ -584,6 +759,10 @@ PyMethodDef g_methods[] = {
     {"set_entry", fast(py_set_entry), METH_FASTCALL, nullptr},
     {"plan_fresh", py_plan_fresh, METH_O, nullptr},
     {"init", fast(py_init), METH_FASTCALL, nullptr},
+    {"kv_write", fast(py_kv_write), METH_FASTCALL, nullptr},
+    {"kv_read", fast(py_kv_read), METH_FASTCALL, nullptr},
+    {"kv_attn", fast(py_kv_attn), METH_FASTCALL, nullptr},
+    {"init_kv", fast(py_init_kv), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

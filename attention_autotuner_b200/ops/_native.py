@@ -25,6 +25,7 @@ TRIES = 16  # attempts at a call that no change of the tuning cache overtakes; e
 
 _lock = threading.Lock()
 _module = None
+_kv_ready = False
 _plans: dict = {}
 _archs: list = []  # device descriptions seen by RetNet calls: the backward resolves its plan with the forward's
 
@@ -57,6 +58,18 @@ def ops():
                      _address(lib.attn_b200_ret_chunk_fwd_ws))
             _module = mod
     return _module
+
+
+def kv_ops():
+    """The native module with the entry points of the KV cache's library (loaded with the first cache)."""
+    global _kv_ready
+    native = ops()
+    if not _kv_ready:
+        lib = _lib.load_kv()
+        native.init_kv(*(_address(getattr(lib, "attn_b200_kv_" + name))
+                         for name in ("last_error", "block_bytes", "write", "read", "attn_workspace_bytes", "attn")))
+        _kv_ready = True
+    return native
 
 
 def _set_entry(plan, tuner, cfg):
