@@ -91,6 +91,26 @@ int kv_sms() {
   return table[dev];
 }
 
+// Every kernel of the cache is launched as a programmatic dependent: its blocks may start while the kernel in front drains, and they
+// wait for its completion before they touch memory.
+template <class Kernel, class... Args>
+int kv_launch(const char* what, Kernel kernel, dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e == cudaSuccess) return kOk;
+  (void)cudaGetLastError();
+  return fail(kErrCuda, "%s: launch: %s", what, cudaGetErrorString(e));
+}
+
 // Always the same limit: calls with other batch sizes on other threads set the attribute too.
 template <class Cfg>
 cudaError_t kv_attn_allow_smem() {
@@ -137,34 +157,12 @@ int kv_attn_launch(KvAttnParams p, size_t ws_bytes, cudaStream_t stream) {
   auto kernel = &kv_attn_kernel<Cfg>;
   cudaError_t e = kv_attn_allow_smem<Cfg>();
   if (e != cudaSuccess) return fail(kErrCuda, "kv_attn: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  // both as programmatic dependents: they wait for what is in front of them in the stream before they read anything
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(Cfg::NTHREADS, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, p);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    return fail(kErrCuda, "kv_attn launch: %s", cudaGetErrorString(e));
-  }
+  if (int rc = kv_launch("kv_attn", kernel, dim3(grid, 1, 1), Cfg::NTHREADS, smem, stream, p)) return rc;
   // tasks of a head: a block of its own for each where there are few heads (one may lie in all runs), a warp where there are many
   const int tasks = std::min(p.rows, Cfg::ROWS) * (Cfg::D / 64);
   const bool few = items * tasks <= 2 * kv_sms();
-  cfg.gridDim = dim3(static_cast<unsigned>(items), static_cast<unsigned>(few ? tasks : (tasks + 7) / 8), 1);
-  cfg.blockDim = dim3(few ? 512 : 256, 1, 1);
-  cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, &kv_attn_join_kernel<Cfg::D, Cfg::ROWS, Cfg::UNIT, Cfg::BF16>, p, grid);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    return fail(kErrCuda, "kv_attn join launch: %s", cudaGetErrorString(e));
-  }
-  return kOk;
+  return kv_launch("kv_attn", &kv_attn_join_kernel<Cfg::D, Cfg::ROWS, Cfg::UNIT, Cfg::BF16>,
+                   dim3(static_cast<unsigned>(items), static_cast<unsigned>(few ? tasks : (tasks + 7) / 8), 1), few ? 512 : 256, 0, stream, p, grid);
 }
 
 template <class F>
@@ -244,8 +242,7 @@ int attn_b200_kv_write(const attn_b200_kv_cache* cache, const int* table, int ta
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return kv_dispatch(cache, [&](auto bits, auto d, auto bf16) {
     const dim3 grid((p.blocks + 3) / 4, p.cache.heads, B);
-    kv_write_kernel<decltype(bits)::value, decltype(d)::value, decltype(bf16)::value><<<grid, 128, 0, st>>>(p);
-    return check_launch("kv_write launch");
+    return kv_launch("kv_write", &kv_write_kernel<decltype(bits)::value, decltype(d)::value, decltype(bf16)::value>, grid, 128, 0, st, p);
   });
 }
 
@@ -266,9 +263,8 @@ int attn_b200_kv_read(const attn_b200_kv_cache* cache, const int* table, int tab
   p.L = L;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return kv_dispatch(cache, [&](auto bits, auto d, auto bf16) {
-    const dim3 grid((L + 4 * kKvBlockTokens - 1) / (4 * kKvBlockTokens), p.cache.heads, B);
-    kv_read_kernel<decltype(bits)::value, decltype(d)::value, decltype(bf16)::value><<<grid, 128, 0, st>>>(p);
-    return check_launch("kv_read launch");
+    const dim3 grid(((L + 2 * kKvBlockTokens - 2) / kKvBlockTokens + 3) / 4, p.cache.heads, B);
+    return kv_launch("kv_read", &kv_read_kernel<decltype(bits)::value, decltype(d)::value, decltype(bf16)::value>, grid, 128, 0, st, p);
   });
 }
 

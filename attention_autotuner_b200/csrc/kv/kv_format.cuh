@@ -105,6 +105,14 @@ struct Kv16<false> {
     const __half2 r = __floats2half2_rn(lo, hi);
     return reinterpret_cast<const uint32_t&>(r);
   }
+  __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b), reinterpret_cast<__half2&>(c));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+  __device__ static __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
   __device__ static __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
     const __half2 r = __hmin2_nan(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
     return reinterpret_cast<const uint32_t&>(r);
@@ -117,6 +125,14 @@ struct Kv16<true> {
   __device__ static __forceinline__ uint32_t round(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
   __device__ static __forceinline__ uint32_t round2(float lo, float hi) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+  __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    const __nv_bfloat162 r = __hfma2(reinterpret_cast<__nv_bfloat162&>(a), reinterpret_cast<__nv_bfloat162&>(b), reinterpret_cast<__nv_bfloat162&>(c));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+  __device__ static __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(reinterpret_cast<__nv_bfloat162&>(a), reinterpret_cast<__nv_bfloat162&>(b));
     return reinterpret_cast<const uint32_t&>(r);
   }
   __device__ static __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {

@@ -1,10 +1,14 @@
 // Quantising K and V of new positions into the pages of a cache (the form: kv_format.cuh), and reading positions back.
 //
 // What bounds both: memory. Writing reads 4 d bytes per position and head and writes 2 (d BITS / 8 + 4); reading back the other
-// way round. A lane owns eight channels (16 bytes of K and of V): d / 8 lanes hold a position, so that the 16-bit side moves in
-// whole rows, minimum and maximum take log2(d / 8) shuffles of a packed pair, and a lane's numbers are one or two words that lie
-// in one piece of a block. A warp owns the (up to) 16 positions of one block of one head: everything it touches of the packed
-// side is one piece of a page.
+// way round. A lane owns eight channels of either half of a row (16 bytes twice, each load of a warp in whole rows); d / 16 lanes
+// hold a position, so that what is done once per row (minimum and maximum by shuffles of a packed pair, two quotients) is
+// shared by 16 channels. A warp owns the 16 positions of one block of one head. It puts them together in shared memory and stores
+// them with one bulk copy if they are all new; a block that is written in part is stored position by position.
+//
+// Next to the memory it is the issue slots that count: at the copy bandwidth an SM has 14 instructions of a lane for each number
+// written, 17 for each read. Hence one fma, two additions and a subtraction for a number (kv_quantise), and the packed fma of
+// the type for a value (kv_values8).
 #pragma once
 
 #include <limits.h>
@@ -32,72 +36,77 @@ struct KvWriteParams {
   int B, L, blocks;   // blocks: of a sequence that L positions can touch
 };
 
-// Eight consecutive channels -> eight numbers of BITS bits. a: x - zero >= 0 in fp32, s: the scale in fp32.
-template <int BITS>
-__device__ __forceinline__ void kv_quantise8(const float* a, float s, uint32_t* out) {
+// Numbers of 16 channels of a row, u: as 16-bit pairs; zero, s, range: of the row, in fp32, range and s finite, s > 0.
+template <int BITS, bool BF16>
+__device__ __forceinline__ void kv_quantise(const uint32_t* u, float zero, float s, float range, uint32_t (*out)[2]) {
+  using T = Kv16<BF16>;
   constexpr float N = static_cast<float>((1 << BITS) - 1);
-  // rint(a / s) by a product: q is off a / s by less than 1e-4 (N times three half steps of fp32), so that its rounding can
-  // only differ next to a half; there the quotient itself decides. (A quotient for each: 20 instructions against 4.)
-  const float inv = 1.0f / s;
-  float n[8];
-  bool near_half = false;
+  constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to whole numbers, half to even
+  const float inv = __frcp_rn(s), c = -zero * inv;
+  // rint((x - zero) / s), its argument by a product: off by less than (1.25 N + 0.75 |c|) 2^-23 (three roundings to 24 bits of numbers
+  // below N, one of c), so that its rounding can only be another next to a half. There, and where numbers could exceed N (a scale
+  // with few bits), the quotient itself decides. (A quotient for every number: 100 instructions more.)
+  const float safe = 0.5f - (1.25f * N + 0.75f * fabsf(c)) * 1.1920929e-7f;
+  float n[16], off = range * inv <= N + 0.25f ? 0.f : 1.f;  // not a number: 1
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = a[i] * inv;
-    n[i] = rintf(q);
-    near_half |= !(fabsf(q - n[i]) <= 0.4999f);  // true for a q that is not a number as well
+  for (int i = 0; i < 16; ++i) {
+    const float q = fmaf(i & 1 ? T::hi(u[i >> 1]) : T::lo(u[i >> 1]), inv, c);
+    n[i] = (q + ROUND) - ROUND;
+    off = fmaxf(off, fabsf(q - n[i]));
   }
-  if (near_half) {
+  if (!(off < safe)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] = rintf(__fdiv_rn(a[i], s));
+    for (int i = 0; i < 16; ++i) n[i] = fminf(rintf(__fdiv_rn((i & 1 ? T::hi(u[i >> 1]) : T::lo(u[i >> 1])) - zero, s)), N);
   }
+  // numbers side by side by sums that are exact in fp32; + 2^23 puts a sum into the low bits
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = fminf(n[i], N);
-  if constexpr (BITS == 4) {
-    // four numbers by sums below 2^16, exact in fp32; + 2^23 puts them into the low bits
-    uint32_t half[2];
+  for (int h = 0; h < 2; ++h) {
+    const float* m = n + 8 * h;
+    if constexpr (BITS == 4) {
+      const uint32_t lo = __float_as_uint(fmaf(m[3], 4096.f, fmaf(m[2], 256.f, fmaf(m[1], 16.f, m[0]))) + 8388608.f);
+      const uint32_t hi = __float_as_uint(fmaf(m[7], 4096.f, fmaf(m[6], 256.f, fmaf(m[5], 16.f, m[4]))) + 8388608.f);
+      out[h][0] = __byte_perm(lo, hi, 0x5410);
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      half[h] = __float_as_uint(fmaf(n[4 * h + 3], 4096.f, fmaf(n[4 * h + 2], 256.f, fmaf(n[4 * h + 1], 16.f, n[4 * h]))) + 8388608.f);
-    out[0] = __byte_perm(half[0], half[1], 0x5410);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t lo = __float_as_uint(fmaf(n[4 * h + 1], 256.f, n[4 * h]) + 8388608.f);
-      const uint32_t hi = __float_as_uint(fmaf(n[4 * h + 3], 256.f, n[4 * h + 2]) + 8388608.f);
-      out[h] = __byte_perm(lo, hi, 0x5410);
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t lo = __float_as_uint(fmaf(m[4 * i + 1], 256.f, m[4 * i]) + 8388608.f);
+        const uint32_t hi = __float_as_uint(fmaf(m[4 * i + 3], 256.f, m[4 * i + 2]) + 8388608.f);
+        out[h][i] = __byte_perm(lo, hi, 0x5410);
+      }
     }
   }
 }
 
-// One row of K or V, eight channels per lane, LANES lanes per row: its numbers, and scale | zero << 16.
+// One row of K or V, eight channels of either half per lane, LANES lanes per row: its numbers, and scale | zero << 16.
 template <int BITS, bool BF16, int LANES>
-__device__ __forceinline__ uint32_t kv_quantise_row(const uint4& x, uint32_t* out) {
+__device__ __forceinline__ uint32_t kv_quantise_row(const uint4* x, uint32_t (*out)[2]) {
   using T = Kv16<BF16>;
-  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  const uint32_t u[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
   constexpr uint32_t SIGNS = 0x80008000u;
-  uint32_t lo = T::min2_nan(T::min2_nan(u[0], u[1]), T::min2_nan(u[2], u[3]));
-  uint32_t hi = T::min2_nan(T::min2_nan(u[0] ^ SIGNS, u[1] ^ SIGNS), T::min2_nan(u[2] ^ SIGNS, u[3] ^ SIGNS));  // of -x
+  uint32_t lo = u[0], hi = u[0] ^ SIGNS;  // minima of x and of -x
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = T::min2_nan(lo, u[i]);
+    hi = T::min2_nan(hi, u[i] ^ SIGNS);
+  }
   uint32_t both = T::min2_nan(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));  // min x | min -x << 16
 #pragma unroll
   for (int m = 1; m < LANES; m <<= 1) both = T::min2_nan(both, __shfl_xor_sync(0xffffffffu, both, m));
   const float zero = T::lo(both), range = -T::hi(both) - zero;
-  const float N = static_cast<float>((1 << BITS) - 1);
-  const uint32_t s16 = T::round(__fdiv_rn(range, N));
+  const uint32_t s16 = T::round(__fdiv_rn(range, static_cast<float>((1 << BITS) - 1)));
   const float s = T::lo(s16);
   if (!(fabsf(range) < INFINITY) || s == 0.f) {  // a row without a finite range, or without one that the type can hold
-    out[0] = 0;
-    if constexpr (BITS == 8) out[1] = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) out[h][0] = out[h][1] = 0;
     return s == 0.f ? (both << 16) : 0x7fff7fffu;  // scale 0; or both NaN
   }
-  float a[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a[2 * i] = T::lo(u[i]) - zero;
-    a[2 * i + 1] = T::hi(u[i]) - zero;
-  }
-  kv_quantise8<BITS>(a, s, out);
+  kv_quantise<BITS, BF16>(u, zero, s, range, out);
   return s16 | (both << 16);
+}
+
+// Untiled bulk copy shared -> global memory; both addresses 16-byte aligned, bytes a multiple of 16.
+__device__ __forceinline__ void kv_bulk_store(void* gmem, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gmem), "r"(smem_u32(smem_src)), "r"(bytes) : "memory");
 }
 
 template <int BITS>
@@ -110,44 +119,65 @@ __device__ __forceinline__ void kv_store_words(uint8_t* to, const uint32_t* w) {
 template <int BITS, int D, bool BF16>
 __global__ void __launch_bounds__(128) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
   using Blk = KvBlock<BITS, D>;
-  constexpr int LANES = D / 8, PER = 32 / LANES;  // lanes per position, positions per instruction
-  constexpr int BATCH = 4;                        // positions in flight per lane
+  constexpr int LANES = D / 16, PER = 32 / LANES;  // lanes per position, positions per instruction
+  __shared__ __align__(128) uint8_t stage[4][Blk::BYTES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, h = blockIdx.y;
+  pdl_grid_dependency_wait();  // launched as a programmatic dependent: what is in front has completed from here on
   const int start = p.start[b];
-  int count = p.count != nullptr ? p.count[b] : p.L;
-  count = kv_count(p.cache, count, start, p.L, b);
+  const int count = kv_count(p.cache, p.count != nullptr ? p.count[b] : p.L, start, p.L, b);
   const int off = (blockIdx.x * 4 + warp) * kKvBlockTokens - start % kKvBlockTokens;  // of this warp's block, from start on
   if (count <= max(off, 0)) return;
   const int pos0 = start + off, first = max(-off, 0), last = min(count - off, kKvBlockTokens);
-  const int page = kv_page(p.cache, b, pos0);
-  if (page < 0) return;
-  uint8_t* blk = kv_block(p.cache, page, h, pos0, Blk::BYTES);
   const int sub = lane / LANES, ch = (lane % LANES) * 8;
   const uint16_t* k = static_cast<const uint16_t*>(p.k) + b * p.k_stride[0] + h * p.k_stride[1] + off * p.k_stride[2] + ch;
   const uint16_t* v = static_cast<const uint16_t*>(p.v) + b * p.v_stride[0] + h * p.v_stride[1] + off * p.v_stride[2] + ch;
-#pragma unroll 1
-  for (int base = first / PER * PER; base < last; base += BATCH * PER) {
-    uint4 kx[BATCH], vx[BATCH];
+  auto load = [&](int tok, uint4* kx, uint4* vx) {
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int tok = base + i * PER + sub;
-      const bool mine = tok >= first && tok < last;
-      kx[i] = mine ? __ldcs(reinterpret_cast<const uint4*>(k + tok * p.k_stride[2])) : make_uint4(0, 0, 0, 0);
-      vx[i] = mine ? __ldcs(reinterpret_cast<const uint4*>(v + tok * p.v_stride[2])) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 2; ++i) {
+      kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+      if (tok >= first && tok < last) {
+        kx[i] = __ldcs(reinterpret_cast<const uint4*>(k + tok * p.k_stride[2] + i * (D / 2)));
+        vx[i] = __ldcs(reinterpret_cast<const uint4*>(v + tok * p.v_stride[2] + i * (D / 2)));
+      }
+    }
+  };
+  const bool whole = first == 0 && last == kKvBlockTokens;
+  const int base0 = first / PER * PER;
+  uint4 kx[2], vx[2], kn[2], vn[2];
+  load(base0 + sub, kx, vx);
+  const int page = kv_page(p.cache, b, pos0);  // beside the first loads
+  if (page < 0) return;
+  uint8_t* blk = kv_block(p.cache, page, h, pos0, Blk::BYTES);
+  uint8_t* to = whole ? stage[warp] : blk;
+#pragma unroll 1
+  for (int base = base0; base < last; base += PER) {
+    const int tok = base + sub;
+    load(tok + PER, kn, vn);
+    uint32_t kw[2][2], vw[2][2];
+    const uint32_t km = kv_quantise_row<BITS, BF16, LANES>(kx, kw);
+    const uint32_t vm = kv_quantise_row<BITS, BF16, LANES>(vx, vw);
+    if (tok >= first && tok < last) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        kv_store_words<BITS>(to + Blk::k_byte(tok, (ch + i * (D / 2)) * BITS / 8), kw[i]);
+        kv_store_words<BITS>(to + Blk::v_byte(tok, (ch + i * (D / 2)) * BITS / 8), vw[i]);
+      }
+      if (ch == 0) *reinterpret_cast<uint2*>(to + Blk::meta_byte(tok)) = make_uint2(km, vm);
     }
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      if (base + i * PER >= last) break;  // the same for all lanes
-      const int tok = base + i * PER + sub;
-      uint32_t kw[2], vw[2];
-      const uint32_t km = kv_quantise_row<BITS, BF16, LANES>(kx[i], kw);
-      const uint32_t vm = kv_quantise_row<BITS, BF16, LANES>(vx[i], vw);
-      if (tok >= first && tok < last) {
-        kv_store_words<BITS>(blk + Blk::k_byte(tok, ch * BITS / 8), kw);
-        kv_store_words<BITS>(blk + Blk::v_byte(tok, ch * BITS / 8), vw);
-        if (ch == 0) *reinterpret_cast<uint2*>(blk + Blk::meta_byte(tok)) = make_uint2(km, vm);
-      }
+    for (int i = 0; i < 2; ++i) {
+      kx[i] = kn[i];
+      vx[i] = vn[i];
+    }
+  }
+  if (whole) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      kv_bulk_store(blk, stage[warp], Blk::BYTES);
+      tma_store_commit();
+      tma_store_wait0();  // it depends on no other thread, and the buffer must outlive it
     }
   }
 }
@@ -161,59 +191,105 @@ struct KvReadParams {
   int B, L;
 };
 
-// Eight numbers -> eight values of the cache's type.
+// Eight numbers -> eight values of the cache's type, each rounded once. meta: scale | zero << 16.
 template <int BITS, bool BF16>
-__device__ __forceinline__ uint4 kv_values8(const uint8_t* from, uint32_t meta) {
+__device__ __forceinline__ uint4 kv_values8(const uint32_t* w, uint32_t meta) {
   using T = Kv16<BF16>;
-  const float s = T::lo(meta), z = T::hi(meta);
-  uint32_t w[2];
-  if constexpr (BITS == 4) w[0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+  if constexpr (BITS == 8 && BF16) {  // 128 + n takes eight bits behind the leading one, and a bf16 has seven
+    const float s = T::lo(meta), z = T::hi(meta);
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float n = __uint_as_float(__byte_perm(w[i >> 1], 0x4b000000u, 0x7440 + 2 * (i & 1) + j)) - 8388608.f;  // 2^23 + n
+        f[j] = fmaf(n, s, z);  // the product is exact, 8 by 8 bits
+      }
+      r[i] = T::round2(f[0], f[1]);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+  } else {
+    // n in the mantissa of 1024 (bf16: 128), an exact difference, and one packed fma
+    constexpr uint32_t BASE = BF16 ? 0x43004300u : 0x64006400u;
+    const uint32_t s2 = __byte_perm(meta, meta, 0x1010), z2 = __byte_perm(meta, meta, 0x3232);
+    uint32_t n[4];
+    if constexpr (BITS == 4) {
+      // nibbles 0 and 4, 1 and 5, ...; put back in order below
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n[i] = ((w[0] >> (4 * i)) & 0x000f000fu) | BASE;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n[i] = __byte_perm(w[i >> 1], BASE, i & 1 ? 0x7372 : 0x7170);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = T::fma2(T::sub2(n[i], BASE), s2, z2);
+    if constexpr (BITS == 8) return make_uint4(n[0], n[1], n[2], n[3]);
+    return make_uint4(__byte_perm(n[0], n[1], 0x5410), __byte_perm(n[2], n[3], 0x5410), __byte_perm(n[0], n[1], 0x7632),
+                      __byte_perm(n[2], n[3], 0x7632));
+  }
+}
+template <int BITS>
+__device__ __forceinline__ void kv_load_words(const uint8_t* from, uint32_t* w) {
+  if constexpr (BITS == 4) w[0] = *reinterpret_cast<const uint32_t*>(from);
   else {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(from));
+    const uint2 x = *reinterpret_cast<const uint2*>(from);
     w[0] = x.x;
     w[1] = x.y;
   }
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t n = BITS == 4 ? (w[0] >> (4 * i)) & 15u : (w[i >> 2] >> (8 * (i & 3))) & 255u;
-    f[i] = fmaf(__uint_as_float(0x4b000000u | n) - 8388608.f, s, z);  // the product is exact: 8 by 11 bits
-  }
-  return make_uint4(T::round2(f[0], f[1]), T::round2(f[2], f[3]), T::round2(f[4], f[5]), T::round2(f[6], f[7]));
 }
 
-// grid (ceil(L / (16 * warps per CTA)), heads, B): a warp owns 16 rows of the output
+// grid (ceil(blocks / warps per CTA), heads, B): a warp owns the positions of a block of the cache
 template <int BITS, int D, bool BF16>
 __global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ KvReadParams p) {
   using Blk = KvBlock<BITS, D>;
-  constexpr int LANES = D / 8, PER = 32 / LANES;
+  constexpr int LANES = D / 16, PER = 32 / LANES, BATCH = 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, h = blockIdx.y;
-  const int row0 = (blockIdx.x * 4 + warp) * kKvBlockTokens;
-  if (row0 >= p.L) return;
-  const int start = p.start != nullptr ? p.start[b] : 0;
-  int count = p.count != nullptr ? p.count[b] : p.L;
-  count = kv_count(p.cache, count, start, p.L, b);
+  pdl_grid_dependency_wait();
+  int start = p.start != nullptr ? p.start[b] : 0;
+  const int count = kv_count(p.cache, p.count != nullptr ? p.count[b] : p.L, start, p.L, b);
+  if (count == 0) start = 0;  // whatever it was
+  const int off = (blockIdx.x * 4 + warp) * kKvBlockTokens - start % kKvBlockTokens;  // of this warp's block, from start on
+  if (off >= p.L) return;
+  const uint8_t* blk = nullptr;
+  if (off < count) {
+    const int page = kv_page(p.cache, b, start + off);
+    if (page >= 0) blk = kv_block(p.cache, page, h, start + off, Blk::BYTES);
+  }
   const int sub = lane / LANES, ch = (lane % LANES) * 8;
-  const long long out0 = ((static_cast<long long>(b) * p.cache.heads + h) * p.L) * D + ch;
-#pragma unroll 4
-  for (int i = 0; i < kKvBlockTokens; i += PER) {
-    const int row = row0 + i + sub;
-    if (row >= p.L) break;
-    uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-    if (row < count) {
-      const int pos = start + row, tok = pos & (kKvBlockTokens - 1);
-      const int page = kv_page(p.cache, b, pos);
-      if (page >= 0) {
-        const uint8_t* blk = kv_block(p.cache, page, h, pos, Blk::BYTES);
-        const uint2 m = __ldg(reinterpret_cast<const uint2*>(blk + Blk::meta_byte(tok)));
-        kx = kv_values8<BITS, BF16>(blk + Blk::k_byte(tok, ch * BITS / 8), m.x);
-        vx = kv_values8<BITS, BF16>(blk + Blk::v_byte(tok, ch * BITS / 8), m.y);
+  const long long out0 = ((static_cast<long long>(b) * p.cache.heads + h) * p.L + off) * D + ch;
+#pragma unroll 1
+  for (int base = 0; base < kKvBlockTokens; base += BATCH * PER) {
+    uint2 meta[BATCH];
+    uint32_t kw[BATCH][2][2], vw[BATCH][2][2];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int tok = base + j * PER + sub;
+      const bool there = blk != nullptr && off + tok >= 0 && off + tok < count;
+      meta[j] = make_uint2(0, 0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kw[j][i][0] = kw[j][i][1] = vw[j][i][0] = vw[j][i][1] = 0;
+      if (there) {
+        meta[j] = *reinterpret_cast<const uint2*>(blk + Blk::meta_byte(tok));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          kv_load_words<BITS>(blk + Blk::k_byte(tok, (ch + i * (D / 2)) * BITS / 8), kw[j][i]);
+          kv_load_words<BITS>(blk + Blk::v_byte(tok, (ch + i * (D / 2)) * BITS / 8), vw[j][i]);
+        }
       }
     }
-    const long long o = out0 + static_cast<long long>(row) * D;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k) + o) = kx;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v) + o) = vx;
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int tok = base + j * PER + sub, row = off + tok;
+      if (row < 0 || row >= p.L) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // scale and zero of a row that is not there are 0, and so are its values
+        const long long o = out0 + static_cast<long long>(tok) * D + i * (D / 2);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k) + o) = kv_values8<BITS, BF16>(kw[j][i], meta[j].x);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v) + o) = kv_values8<BITS, BF16>(vw[j][i], meta[j].y);
+      }
+    }
   }
 }
 
