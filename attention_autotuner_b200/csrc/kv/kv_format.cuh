@@ -117,6 +117,10 @@ struct Kv16<false> {
     const __half2 r = __hmin2_nan(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
     return reinterpret_cast<const uint32_t&>(r);
   }
+  __device__ static __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2_nan(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
 };
 template <>
 struct Kv16<true> {
@@ -137,6 +141,10 @@ struct Kv16<true> {
   }
   __device__ static __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hmin2_nan(reinterpret_cast<__nv_bfloat162&>(a), reinterpret_cast<__nv_bfloat162&>(b));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+  __device__ static __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2_nan(reinterpret_cast<__nv_bfloat162&>(a), reinterpret_cast<__nv_bfloat162&>(b));
     return reinterpret_cast<const uint32_t&>(r);
   }
 };

@@ -7,8 +7,8 @@
 // them with one bulk copy if they are all new; a block that is written in part is stored position by position.
 //
 // Next to the memory it is the issue slots that count: at the copy bandwidth an SM has 14 instructions of a lane for each number
-// written, 17 for each read. Hence one fma, two additions and a subtraction for a number (kv_quantise), and the packed fma of
-// the type for a value (kv_values8).
+// written, 17 for each read. Hence packed fp32 arithmetic for the numbers (kv_quantise) and the packed fma of the type for the values
+// (kv_values8).
 #pragma once
 
 #include <limits.h>
@@ -37,42 +37,61 @@ struct KvWriteParams {
 };
 
 // Numbers of 16 channels of a row, u: as 16-bit pairs; zero, s, range: of the row, in fp32, range and s finite, s > 0.
+// What is rounded to a whole number is the fp32 quotient (x - zero) / s itself, halves included (of bf16 numbers one in 200 is one):
+// q = a inv, then one Newton step q + (a - q s) inv, which gives the quotient rounded to nearest if inv is the reciprocal rounded to
+// nearest and s is not all ones (P. Markstein, IBM J. Res. Dev. 34, 1990); s has 11 bits at most. Two numbers per instruction.
 template <int BITS, bool BF16>
 __device__ __forceinline__ void kv_quantise(const uint32_t* u, float zero, float s, float range, uint32_t (*out)[2]) {
   using T = Kv16<BF16>;
   constexpr float N = static_cast<float>((1 << BITS) - 1);
-  constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to whole numbers, half to even
-  const float inv = __frcp_rn(s), c = -zero * inv;
-  // rint((x - zero) / s), its argument by a product: off by less than (1.25 N + 0.75 |c|) 2^-23 (three roundings to 24 bits of numbers
-  // below N, one of c), so that its rounding can only be another next to a half. There, and where numbers could exceed N (a scale
-  // with few bits), the quotient itself decides. (A quotient for every number: 100 instructions more.)
-  const float safe = 0.5f - (1.25f * N + 0.75f * fabsf(c)) * 1.1920929e-7f;
-  float n[16], off = range * inv <= N + 0.25f ? 0.f : 1.f;  // not a number: 1
+  constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to whole numbers, half to even, in its low bits
+  uint32_t n[16];
+  if (s >= 7.9e-31f && range <= 1.3e30f) {  // 2^-100, 2^100: nothing below leaves the range of fp32
+    const float inv = __frcp_rn(s);
+    const uint64_t inv2 = f2_pack(inv, inv), minus_s2 = f2_pack(-s, -s), minus_zero2 = f2_pack(-zero, -zero), round2 = f2_pack(ROUND, ROUND);
+    uint64_t q[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float q = fmaf(i & 1 ? T::hi(u[i >> 1]) : T::lo(u[i >> 1]), inv, c);
-    n[i] = (q + ROUND) - ROUND;
-    off = fmaxf(off, fabsf(q - n[i]));
-  }
-  if (!(off < safe)) {
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t a = fadd2(f2_pack(T::lo(u[i]), T::hi(u[i])), minus_zero2);
+      const uint64_t q0 = fmul2(a, inv2);
+      q[i] = ffma2(ffma2(q0, minus_s2, a), inv2, q0);
+    }
+    // a scale that was rounded down, by up to half a step of its type, can make the largest number N + 1: of 8 bits and bf16 it
+    // often does and is put right below, else only a subnormal scale is that coarse
+    if ((BITS == 4 || !BF16) && range * inv > N + 0.25f) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) n[i] = fminf(rintf(__fdiv_rn((i & 1 ? T::hi(u[i >> 1]) : T::lo(u[i >> 1])) - zero, s)), N);
+      for (int i = 0; i < 8; ++i) {
+        float x, y;
+        f2_unpack(q[i], x, y);
+        q[i] = f2_pack(fminf(x, N), fminf(y, N));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x, y;
+      f2_unpack(fadd2(q[i], round2), x, y);
+      n[2 * i] = __float_as_uint(x);
+      n[2 * i + 1] = __float_as_uint(y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      n[i] = __float_as_uint(fminf(__fdiv_rn((i & 1 ? T::hi(u[i >> 1]) : T::lo(u[i >> 1])) - zero, s), N) + ROUND);
   }
-  // numbers side by side by sums that are exact in fp32; + 2^23 puts a sum into the low bits
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const float* m = n + 8 * h;
+    const uint32_t* m = n + 8 * h;
     if constexpr (BITS == 4) {
-      const uint32_t lo = __float_as_uint(fmaf(m[3], 4096.f, fmaf(m[2], 256.f, fmaf(m[1], 16.f, m[0]))) + 8388608.f);
-      const uint32_t hi = __float_as_uint(fmaf(m[7], 4096.f, fmaf(m[6], 256.f, fmaf(m[5], 16.f, m[4]))) + 8388608.f);
-      out[h][0] = __byte_perm(lo, hi, 0x5410);
+      uint32_t w = m[7];
+#pragma unroll
+      for (int i = 6; i >= 0; --i) w = (w << 4) + m[i];
+      out[h][0] = w - 0x3f400000u;  // the bits of ROUND, 0x4b400000, shifted by 0, 4, ... and added
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t lo = __float_as_uint(fmaf(m[4 * i + 1], 256.f, m[4 * i]) + 8388608.f);
-        const uint32_t hi = __float_as_uint(fmaf(m[4 * i + 3], 256.f, m[4 * i + 2]) + 8388608.f);
-        out[h][i] = __byte_perm(lo, hi, 0x5410);
-      }
+      for (int i = 0; i < 2; ++i)
+        out[h][i] = BF16 ? __byte_perm(__vminu2(__byte_perm(m[4 * i], m[4 * i + 1], 0x5410), 0x00ff00ffu),
+                                       __vminu2(__byte_perm(m[4 * i + 2], m[4 * i + 3], 0x5410), 0x00ff00ffu), 0x6420)
+                         : __byte_perm(__byte_perm(m[4 * i], m[4 * i + 1], 0x0040), __byte_perm(m[4 * i + 2], m[4 * i + 3], 0x0040), 0x5410);
     }
   }
 }
@@ -83,12 +102,13 @@ __device__ __forceinline__ uint32_t kv_quantise_row(const uint4* x, uint32_t (*o
   using T = Kv16<BF16>;
   const uint32_t u[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
   constexpr uint32_t SIGNS = 0x80008000u;
-  uint32_t lo = u[0], hi = u[0] ^ SIGNS;  // minima of x and of -x
+  uint32_t lo = u[0], hi = u[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
     lo = T::min2_nan(lo, u[i]);
-    hi = T::min2_nan(hi, u[i] ^ SIGNS);
+    hi = T::max2_nan(hi, u[i]);
   }
+  hi ^= SIGNS;
   uint32_t both = T::min2_nan(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));  // min x | min -x << 16
 #pragma unroll
   for (int m = 1; m < LANES; m <<= 1) both = T::min2_nan(both, __shfl_xor_sync(0xffffffffu, both, m));
