@@ -259,56 +259,68 @@ __device__ __forceinline__ void kv_load_words(const uint8_t* from, uint32_t* w) 
   }
 }
 
-// grid (ceil(blocks / warps per CTA), heads, B): a warp owns the positions of a block of the cache
+enum KvReadTag : int { kTagKvRead = 103 };
+
+// grid (ceil(blocks / warps per CTA), heads, B): a warp owns the positions of a block of the cache, which one bulk copy brings
 template <int BITS, int D, bool BF16>
 __global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ KvReadParams p) {
   using Blk = KvBlock<BITS, D>;
-  constexpr int LANES = D / 16, PER = 32 / LANES, BATCH = 2;
+  constexpr int LANES = D / 16, PER = 32 / LANES;
+  __shared__ __align__(128) uint8_t stage[4][Blk::BYTES];
+  __shared__ uint64_t full[4];
+  __shared__ CtaAbort abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, h = blockIdx.y;
+  if (lane == 0) mbar_init(&full[warp], 1);
+  abort_flag.flag = 0;  // every thread the same; another warp sets it only for a wait that ran out, a second later
+  fence_mbar_init();
+  __syncwarp();
   pdl_grid_dependency_wait();
   int start = p.start != nullptr ? p.start[b] : 0;
   const int count = kv_count(p.cache, p.count != nullptr ? p.count[b] : p.L, start, p.L, b);
   if (count == 0) start = 0;  // whatever it was
   const int off = (blockIdx.x * 4 + warp) * kKvBlockTokens - start % kKvBlockTokens;  // of this warp's block, from start on
   if (off >= p.L) return;
-  const uint8_t* blk = nullptr;
+  bool there = false;  // the same for the warp
   if (off < count) {
     const int page = kv_page(p.cache, b, start + off);
-    if (page >= 0) blk = kv_block(p.cache, page, h, start + off, Blk::BYTES);
+    there = page >= 0;
+    if (there && lane == 0) {
+      mbar_expect_tx(&full[warp], Blk::BYTES);
+      bulk_load_1d(stage[warp], kv_block(p.cache, page, h, start + off, Blk::BYTES), Blk::BYTES, &full[warp]);
+    }
+    __syncwarp();
+    if (there && !mbar_wait_warp(&full[warp], 0, &abort_flag, kTagKvRead)) {
+      if (lane == 0) mbar_wait_drain(&full[warp], 0, 2000000ull);
+      return;
+    }
   }
+  const uint8_t* blk = stage[warp];
   const int sub = lane / LANES, ch = (lane % LANES) * 8;
   const long long out0 = ((static_cast<long long>(b) * p.cache.heads + h) * p.L + off) * D + ch;
-#pragma unroll 1
-  for (int base = 0; base < kKvBlockTokens; base += BATCH * PER) {
-    uint2 meta[BATCH];
-    uint32_t kw[BATCH][2][2], vw[BATCH][2][2];
+#pragma unroll 2
+  for (int base = 0; base < kKvBlockTokens; base += PER) {
+    const int tok = base + sub, row = off + tok;
+    if (row < 0 || row >= p.L) continue;
+    uint4 k[2], v[2];
+    if (there && row < count) {
+      const uint2 meta = *reinterpret_cast<const uint2*>(blk + Blk::meta_byte(tok));
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const int tok = base + j * PER + sub;
-      const bool there = blk != nullptr && off + tok >= 0 && off + tok < count;
-      meta[j] = make_uint2(0, 0);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) kw[j][i][0] = kw[j][i][1] = vw[j][i][0] = vw[j][i][1] = 0;
-      if (there) {
-        meta[j] = *reinterpret_cast<const uint2*>(blk + Blk::meta_byte(tok));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          kv_load_words<BITS>(blk + Blk::k_byte(tok, (ch + i * (D / 2)) * BITS / 8), kw[j][i]);
-          kv_load_words<BITS>(blk + Blk::v_byte(tok, (ch + i * (D / 2)) * BITS / 8), vw[j][i]);
-        }
+      for (int i = 0; i < 2; ++i) {
+        uint32_t kw[2], vw[2];
+        kv_load_words<BITS>(blk + Blk::k_byte(tok, (ch + i * (D / 2)) * BITS / 8), kw);
+        kv_load_words<BITS>(blk + Blk::v_byte(tok, (ch + i * (D / 2)) * BITS / 8), vw);
+        k[i] = kv_values8<BITS, BF16>(kw, meta.x);
+        v[i] = kv_values8<BITS, BF16>(vw, meta.y);
       }
+    } else {
+      k[0] = k[1] = v[0] = v[1] = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const int tok = base + j * PER + sub, row = off + tok;
-      if (row < 0 || row >= p.L) continue;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // scale and zero of a row that is not there are 0, and so are its values
-        const long long o = out0 + static_cast<long long>(tok) * D + i * (D / 2);
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k) + o) = kv_values8<BITS, BF16>(kw[j][i], meta[j].x);
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v) + o) = kv_values8<BITS, BF16>(vw[j][i], meta[j].y);
-      }
+    for (int i = 0; i < 2; ++i) {
+      const long long o = out0 + static_cast<long long>(tok) * D + i * (D / 2);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k) + o) = k[i];
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v) + o) = v[i];
     }
   }
 }
