@@ -48,7 +48,7 @@ struct KvAttnConfig {
   static constexpr int UNIT_BLOCKS = Blk::BYTES <= 2176 ? 2 : 1;  // a unit of work, and of the ring
   static constexpr int UNIT = UNIT_BLOCKS * kKvBlockTokens;       // positions
   static constexpr int UNIT_BYTES = UNIT_BLOCKS * Blk::BYTES;
-  static constexpr int NSTAGE = UNIT_BYTES <= 2304 ? 4 : UNIT_BYTES <= 4352 ? 3 : 2;
+  static constexpr int NSTAGE = UNIT_BYTES <= 2304 ? 4 : 2;
   static constexpr int RING_BYTES = NWARPS * NSTAGE * UNIT_BYTES;
   static constexpr int PART_STRIDE = D + 4;  // floats of a row: the rows of a warp's store fall on other banks
   static constexpr int STAT_BYTES = 3 * NWARPS * ROWS * 4;  // reference, sum, sum of p vz
@@ -124,38 +124,21 @@ __device__ __forceinline__ uint32_t kv_transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// K: whole numbers as fp16 bit patterns. n in the low bits of a half is the subnormal n 2^-24, which the tensor cores take as that;
-// a nibble four bits higher is n 2^-20. (They line a subnormal up as if its leading bit were set and drop what lies below the same
-// place as for a number with that bit: n 2^-24 loses ten bits of some 28, which a score does not notice.)
-constexpr float kKvLoUnit = 16777216.f;  // 2^24
+// Whole numbers as fp16 bit patterns: n in the low bits of a half is the subnormal n 2^-24, which the tensor cores take as that; a
+// nibble four bits higher is n 2^-20.
+constexpr float kKvLoUnit = 16777216.f, kKvHiUnit = 1048576.f;  // 2^24, 2^20
 __device__ __forceinline__ uint32_t kv_nibble_lo(uint32_t x) { return x & 0x000f000fu; }  // nibbles 0 and 4
 __device__ __forceinline__ uint32_t kv_nibble_hi(uint32_t x) { return x & 0x00f000f0u; }  // nibbles 1 and 5, times 16
+// The tensor cores line a subnormal up as if its leading bit were set, and drop what lies below the same place as for a number with
+// that bit. Of the even channels of V, n 2^-24 with n < 16, that is seen in an fp16 output: there it is n 2^-14.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t kv_even(uint32_t x) {
+  if constexpr (!EXACT) return x;
+  const uint32_t up = 0x64006400u;  // 2^10
+  const __half2 r = __hmul2(reinterpret_cast<__half2&>(x), reinterpret_cast<const __half2&>(up));
+  return reinterpret_cast<const uint32_t&>(r);
+}
 __device__ __forceinline__ uint32_t kv_bytes(uint32_t x, uint32_t sel) { return __byte_perm(x, 0, sel); }
-
-// V: whole numbers counted from the middle, exactly, as fp16: the number goes into the mantissa of 1024. The accumulators of O^T
-// run over a whole sequence, and the tensor cores drop the bits that do not fit, always the same way: counted from 0, the
-// sums are large and cancel against that of the zeros (131072 positions: 7e-3 off), counted from the middle they stay small.
-__device__ __forceinline__ uint32_t kv_hadd2(uint32_t a, uint32_t b) {
-  const __half2 r = __hadd2(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
-  return reinterpret_cast<const uint32_t&>(r);
-}
-__device__ __forceinline__ uint32_t kv_hfma2(uint32_t a, uint32_t b, uint32_t c) {
-  const __half2 r = __hfma2(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b), reinterpret_cast<__half2&>(c));
-  return reinterpret_cast<const uint32_t&>(r);
-}
-// (c is 0x64006400 from a register that the compiler does not see into: with two constants in an instruction it makes two.)
-__device__ __forceinline__ uint32_t kv_and_or(uint32_t x, uint32_t mask, uint32_t c) {
-  uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(mask), "r"(c));
-  return y;
-}
-__device__ __forceinline__ uint32_t kv_mid_lo(uint32_t x, uint32_t c) { return kv_hadd2(kv_and_or(x, 0x000f000fu, c), 0xe408e408u); }  // - 1032
-__device__ __forceinline__ uint32_t kv_mid_hi(uint32_t x, uint32_t c) {  // (1024 + 16 n) / 16 - 72
-  return kv_hfma2(kv_and_or(x, 0x00f000f0u, c), 0x2c002c00u, 0xd480d480u);
-}
-__device__ __forceinline__ uint32_t kv_mid_bytes(uint32_t x, uint32_t sel) {  // - 1152
-  return kv_hadd2(__byte_perm(x, 0x64646464u, sel), 0xe480e480u);
-}
 
 // Over the lanes that work on the same rows: those of one t, with HALF of t and t ^ 2.
 template <bool HALF>
@@ -187,8 +170,9 @@ struct KvAttnState {
   int lim[NT][2];              // keys that the row of the column may see
   float m[NT][2], l[NT][2], z[NT][2];
   float acc[D / 16][NT][4];
-  uint32_t c1024;              // two fp16 1024
-  float vup, vdown, vmax;      // scales of V are used times vup, a power of two; they may reach vmax; vdown = 1 / vup
+  float vflip;                 // 0, or 2^bits - 1 for a lane whose positions are odd: their numbers of V are stored as that minus n
+  // scales of V are used times vup, a power of two and the sign of the lane's positions; they may reach vmax; vdown = 1 / |vup|
+  float vup, vdown, vmax;
 };
 
 // The query rows row0 ... of a head, a thread eight channels: fetched early, stored as the fragments of all warps.
@@ -297,11 +281,10 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
   const int g = lane >> 2;
 
   constexpr int R = Cfg::R;
-  constexpr float MID = static_cast<float>(1 << (BITS - 1));
   const int own = Cfg::HALF ? (lane & 2) * 4 : 0;  // the first position of this lane is g + own
 
   float s[NB][NT][2 * R];
-  float ks[NB][R], kz[NB][R], vs[NB][R], vz[NB][R];  // of the lane's positions; vz: the value of the middle number
+  float ks[NB][R], kz[NB][R], vs[NB][R], vz[NB][R];  // of the lane's positions; vz: what V stands for with its numbers 0
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const uint8_t* at = blk + nb * Blk::BYTES;
@@ -314,7 +297,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
       ks[nb][r] = T::lo(meta.x);
       kz[nb][r] = T::hi(meta.x);
       vs[nb][r] = T::lo(meta.y);
-      vz[nb][r] = fmaf(MID, vs[nb][r], T::hi(meta.y));
+      vz[nb][r] = fmaf(st.vflip, vs[nb][r], T::hi(meta.y));
     }
     uint32_t w[LANE_UNITS * 4];
 #pragma unroll
@@ -415,7 +398,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 6 - x) << 23);
       const float f = up * st.vdown;
       st.vmax = __uint_as_float(static_cast<uint32_t>(127 + min(x + 4, 127)) << 23);
-      st.vup = up;
+      st.vup = st.vflip != 0.f ? -up : up;
       st.vdown = __uint_as_float(static_cast<uint32_t>(127 - 6 + x) << 23);
 #pragma unroll
       for (int u = 0; u < D / 16; ++u)
@@ -486,15 +469,15 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         uint32_t f[4];
         if constexpr (BITS == 4) {
           const uint32_t p0 = i & 1 ? ab[i >> 1] >> 8 : ab[i >> 1], p1 = i & 1 ? cd[i >> 1] >> 8 : cd[i >> 1];
-          f[0] = kv_mid_lo(p0, st.c1024);
-          f[1] = kv_mid_hi(p0, st.c1024);
-          f[2] = kv_mid_lo(p1, st.c1024);
-          f[3] = kv_mid_hi(p1, st.c1024);
+          f[0] = kv_even<Cfg::SPLIT>(kv_nibble_lo(p0));
+          f[1] = kv_nibble_hi(p0);
+          f[2] = kv_even<Cfg::SPLIT>(kv_nibble_lo(p1));
+          f[3] = kv_nibble_hi(p1);
         } else {
-          f[0] = kv_mid_bytes(ab[i], 0x4240);
-          f[1] = kv_mid_bytes(ab[i], 0x4341);
-          f[2] = kv_mid_bytes(cd[i], 0x4240);
-          f[3] = kv_mid_bytes(cd[i], 0x4341);
+          f[0] = kv_bytes(ab[i], 0x4240);
+          f[1] = kv_bytes(ab[i], 0x4341);
+          f[2] = kv_bytes(cd[i], 0x4240);
+          f[3] = kv_bytes(cd[i], 0x4341);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -701,7 +684,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
   bool ok = true;
   int k = 0, slot = 0, phase = 0;  // units of this warp that are done; where the next one is
   KvAttnState<Cfg> st;
-  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(st.c1024));
+  st.vflip = (lane >> 2) & 1 ? static_cast<float>((1 << Cfg::BITS) - 1) : 0.f;
   for (int done = 0;;) {  // units of the run before this head
     kv_begin<Cfg>(st, qs, lane);
     const int clear = p.causal ? cur.len - p.Lq + 1 : cur.len;  // positions below this are seen by every row
@@ -737,6 +720,8 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     // the four warps' partial results
     const int g = lane >> 2, t = lane & 3;
     const int nrows = min(ROWS, p.rows - cur.row0);
+    // what the numbers were taken for: odd channels of 4 bits times 16
+    const float even = st.vdown * (Cfg::BITS == 4 && Cfg::SPLIT ? 16384.f : kKvLoUnit), odd = st.vdown * (Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -759,8 +744,8 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
           float* dst = part + (warp * part_rows + row) * PS + g * (D / 8);
 #pragma unroll
           for (int u = 0; u < D / 16; u += 2)
-            *reinterpret_cast<float4*>(dst + 2 * u) = make_float4(st.acc[u][nt][c] * st.vdown, st.acc[u][nt][2 + c] * st.vdown,
-                                                                  st.acc[u + 1][nt][c] * st.vdown, st.acc[u + 1][nt][2 + c] * st.vdown);
+            *reinterpret_cast<float4*>(dst + 2 * u) = make_float4(st.acc[u][nt][c] * even, st.acc[u][nt][2 + c] * odd,
+                                                                  st.acc[u + 1][nt][c] * even, st.acc[u + 1][nt][2 + c] * odd);
         }
       }
     __syncthreads();
@@ -882,6 +867,13 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
     for (int task = blockIdx.y + gridDim.y * warp; task < tasks; task += gridDim.y * NW) {
       const int row = task / PAIRS, pair = task % PAIRS;
       float m[2], l[2], M = -INFINITY, L = 0.f;
+      float2 y[8];
+      auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i0 + j < parts) y[j] = reinterpret_cast<const float2*>(part_at(i0 + j) + row * D)[pair * 32 + lane];
+      };
+      fetch(0);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const bool there = lane + 32 * j < parts;
@@ -901,10 +893,7 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
       for (int k = 1; k < 32; k <<= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
       float2 x = make_float2(0.f, 0.f);
       for (int i0 = 0; i0 < parts; i0 += 8) {
-        float2 y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (i0 + j < parts) y[j] = reinterpret_cast<const float2*>(part_at(i0 + j) + row * D)[pair * 32 + lane];
+        if (i0 > 0) fetch(i0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float w = __shfl_sync(0xffffffffu, i0 < 32 ? m[0] : m[1], i0 + j);

@@ -177,9 +177,12 @@ __global__ void __launch_bounds__(128) kv_write_kernel(const __grid_constant__ K
     uint32_t kw[2][2], vw[2][2];
     const uint32_t km = kv_quantise_row<BITS, BF16, LANES>(kx, kw);
     const uint32_t vm = kv_quantise_row<BITS, BF16, LANES>(vx, vw);
+    const uint32_t flip = tok & 1 ? ~0u : 0u;  // V of odd positions: 2^BITS - 1 - n
     if (tok >= first && tok < last) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        vw[i][0] ^= flip;
+        vw[i][1] ^= flip;
         kv_store_words<BITS>(to + Blk::k_byte(tok, (ch + i * (D / 2)) * BITS / 8), kw[i]);
         kv_store_words<BITS>(to + Blk::v_byte(tok, (ch + i * (D / 2)) * BITS / 8), vw[i]);
       }
@@ -305,11 +308,14 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ Kv
     uint4 k[2], v[2];
     if (there && row < count) {
       const uint2 meta = *reinterpret_cast<const uint2*>(blk + Blk::meta_byte(tok));
+      const uint32_t flip = tok & 1 ? ~0u : 0u;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t kw[2], vw[2];
+        uint32_t kw[2], vw[2] = {0, 0};
         kv_load_words<BITS>(blk + Blk::k_byte(tok, (ch + i * (D / 2)) * BITS / 8), kw);
         kv_load_words<BITS>(blk + Blk::v_byte(tok, (ch + i * (D / 2)) * BITS / 8), vw);
+        vw[0] ^= flip;
+        vw[1] ^= flip;
         k[i] = kv_values8<BITS, BF16>(kw, meta.x);
         v[i] = kv_values8<BITS, BF16>(vw, meta.y);
       }
