@@ -119,7 +119,7 @@ def _declare_kv(lib):
             ("status", ci, [ci]), ("prepare", ci, []), ("block_bytes", ci, [ci, ci]),
             ("write", ci, [cs, vp, ci, ci, vp, vp, vp, strides, vp, strides, ci, ci, vp]),
             ("read", ci, [cs, vp, ci, ci, vp, vp, vp, vp, ci, ci, vp]),
-            ("attn_workspace_bytes", ctypes.c_size_t, [cs, ci, ci, ci]),
+            ("attn_workspace_bytes", ctypes.c_size_t, [cs, ci, ci, ci, ci]),
             ("attn", ci, [vp, cs, vp, ci, ci, vp, vp, vp, vp, ctypes.c_size_t, ci, ci, ci, ctypes.c_float, ci, vp])):
         fn = getattr(lib, "attn_b200_kv_" + name)
         fn.restype, fn.argtypes = res, args

@@ -654,12 +654,11 @@ PyObject* py_kv_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int B = i32(q.size(0)), group = i32(q.size(1) / c.c.heads), Lq = i32(q.size(2));
     o = at::empty(q.sizes(), q.options());
     if (ret_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-    const size_t bytes = g_kv.attn_ws(&c.c, B, group, Lq);
+    const size_t bytes = g_kv.attn_ws(&c.c, i32(rows.size(1)), B, group, Lq);
     Tensor ws;
     if (bytes != 0) ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
-    // without a workspace the sizes are not supported: the library says which
     check_kv_rc(g_kv.attn(ptr(qc), &c.c, rows.const_data_ptr<int>(), table_stride(rows), i32(rows.size(1)), len.const_data_ptr<int>(), ptr(o),
-                          static_cast<float*>(ptr(lse)), bytes != 0 ? ptr(ws) : ptr(o), bytes, B, group, Lq, static_cast<float>(scale),
+                          static_cast<float*>(ptr(lse)), ptr(ws), bytes, B, group, Lq, static_cast<float>(scale),
                           causal, stream_of(c.data)));
   }
   if (!ret_lse) return THPVariable_Wrap(std::move(o));

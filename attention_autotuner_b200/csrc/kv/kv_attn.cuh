@@ -68,6 +68,7 @@ struct KvAttnParams {
   float* lse;          // or nullptr
   float* ws;           // 2 slots per CTA
   int B, Lq, rows, row_blocks, causal;
+  int whole;           // runs begin where heads begin: nothing to add afterwards
   FastDiv by_grid;     // of the attention kernel, for both
   float scale_log2;
 };
@@ -596,7 +597,8 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int b = find(costs, cost);
     const int n = pre[b + 1] - pre[b];
     const int rem = cost - costs[b] * per_seq, item = kv_div(rem, n + kKvHeadCost);
-    return pre[b] * per_seq + item * n + max(rem - item * (n + kKvHeadCost) - kKvHeadCost, 0);
+    const int in_head = rem - item * (n + kKvHeadCost);
+    return pre[b] * per_seq + item * n + (p.whole ? (in_head > 0 ? n : 0) : max(in_head - kKvHeadCost, 0));
   };
   const int t0 = units_before(range.first(blockIdx.x)), t1 = units_before(range.first(blockIdx.x + 1));
   const int mine = t1 - t0;

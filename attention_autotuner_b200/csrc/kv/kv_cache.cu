@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <array>
+#include <atomic>
 
 #include "../host_common.cuh"
 #include "kv_attn.cuh"
@@ -111,10 +112,18 @@ int kv_launch(const char* what, Kernel kernel, dim3 grid, int threads, int smem,
   return fail(kErrCuda, "%s: launch: %s", what, cudaGetErrorString(e));
 }
 
-// Always the same limit: calls with other batch sizes on other threads set the attribute too.
+// Once per device; always the same limit, whatever the batch.
 template <class Cfg>
 cudaError_t kv_attn_allow_smem() {
-  return cudaFuncSetAttribute(&kv_attn_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::ROWS, kKvMaxBatch));
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(&kv_attn_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::ROWS, kKvMaxBatch));
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // CTAs of a launch: as many as the GPU holds at once (with the prefix sums of an ordinary batch).
@@ -136,8 +145,17 @@ int kv_attn_grid(int rows) {
   return std::min(per_sm[rows < Cfg::ROWS ? rows : Cfg::ROWS] * kv_sms(), kKvMaxRuns);
 }
 
+// Heads of few positions are not split, which saves the second kernel: a quarter of a head's units, one after another, then
+// take less than the parts' way through memory. With tables of 128 / 256 / 512 / 768 positions, a call split and whole, us:
+//   2 x 4 heads, d = 64, 4 bits   5.2  4.3 |  5.8  5.1 |  6.7  6.4 |  6.7  7.7
+//   16 x 8 heads, d = 128, 4 bits 6.1  5.6 |  8.3  7.4 |  9.4 10.3 | 10.6 13.0
+//   64 x 8 heads, d = 128, 4 bits 11.0 9.4 | 13.5 12.1 | 17.3 17.5 | 20.5 22.6
+//   8 x 8 heads, d = 128, 8 bits  6.2  5.6 |  7.4  6.9 |  8.5 10.4 |  8.9 13.5
+bool kv_attn_whole(long long positions, int d) { return positions * d <= 512 * 64; }
+
 template <class Cfg>
-size_t kv_attn_ws_bytes(int rows) {
+size_t kv_attn_ws_bytes(int rows, long long positions) {
+  if (kv_attn_whole(positions, Cfg::D)) return 0;
   return static_cast<size_t>(2) * kv_attn_grid<Cfg>(rows) * Cfg::ROWS * (Cfg::D + 2) * sizeof(float);
 }
 
@@ -150,14 +168,17 @@ int kv_attn_launch(KvAttnParams p, size_t ws_bytes, cudaStream_t stream) {
     return fail(kErrInvalidArgument, "kv_attn: %d sequences x %d heads x %d row blocks with tables of %d pages exceed 2^31 units of work", p.B,
                 p.cache.heads, p.row_blocks, p.cache.table_width);
   const int grid = kv_attn_grid<Cfg>(p.rows);
-  if (ws_bytes < kv_attn_ws_bytes<Cfg>(p.rows))
-    return fail(kErrInvalidArgument, "kv_attn: %zu bytes of workspace, %zu are needed", ws_bytes, kv_attn_ws_bytes<Cfg>(p.rows));
+  const size_t need = kv_attn_ws_bytes<Cfg>(p.rows, static_cast<long long>(p.cache.table_width) << p.cache.page_shift);
+  if (ws_bytes < need || (need > 0 && p.ws == nullptr))
+    return fail(kErrInvalidArgument, "kv_attn: %zu bytes of workspace, %zu are needed", p.ws == nullptr ? size_t(0) : ws_bytes, need);
   const int smem = Cfg::smem_bytes(p.rows, p.B);
   p.by_grid = make_fast_div(grid);
+  p.whole = kv_attn_whole(static_cast<long long>(p.cache.table_width) << p.cache.page_shift, Cfg::D);
   auto kernel = &kv_attn_kernel<Cfg>;
   cudaError_t e = kv_attn_allow_smem<Cfg>();
   if (e != cudaSuccess) return fail(kErrCuda, "kv_attn: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   if (int rc = kv_launch("kv_attn", kernel, dim3(grid, 1, 1), Cfg::NTHREADS, smem, stream, p)) return rc;
+  if (p.whole) return kOk;
   // tasks of a head: a block of its own for each where there are few heads (one may lie in all runs), a warp where there are many
   const int tasks = std::min(p.rows, Cfg::ROWS) * (Cfg::D / 64);
   const bool few = items * tasks <= 2 * kv_sms();
@@ -268,11 +289,11 @@ int attn_b200_kv_read(const attn_b200_kv_cache* cache, const int* table, int tab
   });
 }
 
-size_t attn_b200_kv_attn_workspace_bytes(const attn_b200_kv_cache* cache, int B, int group, int Lq) {
-  if (!kv_attn_sizes_ok(cache, B, group, Lq)) return 0;
+size_t attn_b200_kv_attn_workspace_bytes(const attn_b200_kv_cache* cache, int table_width, int B, int group, int Lq) {
+  if (!kv_attn_sizes_ok(cache, B, group, Lq) || table_width <= 0) return 0;
   size_t bytes = 0;
   kv_attn_dispatch(cache, group * Lq, [&](auto cfg) {
-    bytes = kv_attn_ws_bytes<decltype(cfg)>(group * Lq);
+    bytes = kv_attn_ws_bytes<decltype(cfg)>(group * Lq, static_cast<long long>(table_width) * cache->page_size);
     return 0;
   });
   return bytes;
@@ -283,7 +304,7 @@ int attn_b200_kv_attn(const void* q, const attn_b200_kv_cache* cache, const int*
                       float scale, int causal, void* stream) {
   KvAttnParams p{};
   if (int rc = kv_view(&p.cache, cache, table, table_stride, table_width, B, "kv_attn")) return rc;
-  if (q == nullptr || o == nullptr || lengths == nullptr || workspace == nullptr) return fail(kErrInvalidArgument, "kv_attn: null pointer");
+  if (q == nullptr || o == nullptr || lengths == nullptr) return fail(kErrInvalidArgument, "kv_attn: null pointer");
   if (!kv_attn_sizes_ok(cache, B, group, Lq))
     return fail(kErrInvalidArgument, "kv_attn: %d sequences (at most %d), %d query heads per head of the cache, %d queries (at most %d)", B,
                 kKvMaxBatch, group, Lq, ATTN_B200_KV_MAX_QUERIES);

@@ -471,6 +471,14 @@ def test_refusals_on_the_device():
     for length in (0, -1, 1.5, True, None):
         with pytest.raises(ValueError, match="length"):
             kv_cache_read(cache, table, length=length)
+    # the C ABI: a workspace that is missing, too small or misaligned
+    import ctypes
+    lib, c, big = _lib.load_kv(), cache.struct(), torch.zeros(1, 64, dtype=torch.int32, device="cuda")
+    need = lib.attn_b200_kv_attn_workspace_bytes(ctypes.byref(c), 64, 1, 2, 1)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    for at, size in ((None, 0), (None, need), (ws.data_ptr(), need - 1), (ws.data_ptr() + 8, need)):
+        assert lib.attn_b200_kv_attn(q.data_ptr(), ctypes.byref(c), big.data_ptr(), 64, 64, lengths.data_ptr(), q.data_ptr(), None, at, size, 1, 2, 1,
+                                     0.125, 0, torch.cuda.current_stream().cuda_stream) == 1
     many = torch.zeros(4097, 1, dtype=torch.int32, device="cuda")
     with pytest.raises(_lib.AttnB200Error, match="4097"):
         kv_cache_attn(q.expand(4097, 4, 1, 64), cache, many, torch.zeros(4097, dtype=torch.int32, device="cuda"))

@@ -61,10 +61,14 @@ def test_the_library_checks_before_it_looks_for_a_device():
         c = _lib.KVCacheStruct(**good)
         return lib.attn_b200_kv_attn(q, ctypes.byref(c), 64, table_width, table_width, 64, 64, None, ws, 0, B, group, Lq, scale, 0, None)
 
+    # no workspace for tables of few positions, nor for sizes that are refused
+    c = _lib.KVCacheStruct(**good)
+    assert lib.attn_b200_kv_attn_workspace_bytes(ctypes.byref(c), 2, 1, 1, 1) == 0
+    assert lib.attn_b200_kv_attn_workspace_bytes(ctypes.byref(c), 200, 0, 1, 1) == 0
     odd = (ctypes.c_longlong * 3)(0, 64, 63)
     for rc in (write(data=None), write(data=72), write(bits=5), write(head_dim=80), write(page_size=24), write(num_pages=0), write(dtype=2),
                write(table=None), write(stride=1), write(width=1 << 28, stride=1 << 28), write(k=None), write(k=66), write(strides=odd),
-               write(B=0), write(B=65536), write(L=0), attn(q=None), attn(q=72), attn(ws=None), attn(B=4097), attn(group=0), attn(Lq=65),
+               write(B=0), write(B=65536), write(L=0), attn(q=None), attn(q=72), attn(ws=72), attn(B=4097), attn(group=0), attn(Lq=65),
                attn(scale=0.0), attn(scale=float("nan"))):
         assert rc in (1, 2), rc
         assert lib.attn_b200_kv_last_error().decode().startswith("kv_")
