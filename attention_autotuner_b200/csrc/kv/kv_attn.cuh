@@ -28,8 +28,6 @@
 
 namespace ab200 {
 
-enum KvAttnTag : int { kTagKvFull = 101 };
-
 constexpr int kKvMaxBatch = 4096;  // prefix sums of the work in shared memory
 
 template <int BITS_, int D_, int ROWS_, bool BF16_>
@@ -54,10 +52,9 @@ struct KvAttnConfig {
   static constexpr int STAT_BYTES = 3 * NWARPS * ROWS * 4;  // reference, sum, sum of p vz
   static constexpr int Q_BYTES = 8 * NT * (D * 2 + 16);  // fragments, and what kv_store_q says of a row
   static constexpr int Q_PASSES = (ROWS * D / 8 + NTHREADS - 1) / NTHREADS;
-  static constexpr int BAR_BYTES = 256;
   static constexpr int MIN_CTAS = NT * D <= 64 || ROWS * D <= 512 ? 3 : NT * D <= 128 ? 3 : 2;  // 128, 168 or 255 registers
   static constexpr int part_bytes(int rows) { return NWARPS * (rows < ROWS ? rows : ROWS) * PART_STRIDE * 4; }
-  static int smem_bytes(int rows, int B) { return RING_BYTES + Q_BYTES + STAT_BYTES + BAR_BYTES + part_bytes(rows) + (B + 1) * 8; }
+  static int smem_bytes(int rows, int B) { return RING_BYTES + Q_BYTES + STAT_BYTES + part_bytes(rows) + (B + 1) * 8; }
 };
 
 struct KvAttnParams {
@@ -119,6 +116,10 @@ __device__ __forceinline__ void kv_mma(float* d, const uint32_t* a, const uint32
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// 16 bytes from global to shared memory; both addresses multiples of 16.
+__device__ __forceinline__ void kv_copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t kv_transpose8x8(uint32_t x) {
   uint32_t y;
@@ -499,13 +500,9 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* qs = smem + Cfg::RING_BYTES;                                         // kv_store_q
   float* stat = reinterpret_cast<float*>(qs + Cfg::Q_BYTES);                    // [3][NW][ROWS]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(qs + Cfg::Q_BYTES + Cfg::STAT_BYTES);  // [NW][NSTAGE]
-  int* miss = reinterpret_cast<int*>(bars + NW * NSTAGE);                       // [NW][NSTAGE]: blocks of a unit that are in no page
-  CtaAbort* ab = reinterpret_cast<CtaAbort*>(miss + NW * NSTAGE);
-  static_assert(NW * NSTAGE * 12 + 8 <= Cfg::BAR_BYTES, "barriers, flags, scan");
   __shared__ int scan[2][NW];
   const int part_rows = min(ROWS, p.rows);
-  float* part = reinterpret_cast<float*>(qs + Cfg::Q_BYTES + Cfg::STAT_BYTES + Cfg::BAR_BYTES);  // [NW][part_rows][PS]
+  float* part = reinterpret_cast<float*>(qs + Cfg::Q_BYTES + Cfg::STAT_BYTES);  // [NW][part_rows][PS]
   int* pre = reinterpret_cast<int*>(part + NW * part_rows * PS);  // [B + 1]: units of the sequences before, for one head and row block
   int* costs = pre + p.B + 1;                                     // [B + 1]: the same with the heads' cost
 
@@ -514,9 +511,6 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
   const int per_seq = p.cache.heads * p.row_blocks;
 
   pdl_launch_dependents();
-  if (threadIdx.x < NW * NSTAGE) mbar_init(&bars[threadIdx.x], 1);
-  if (threadIdx.x == 0) ab->flag = 0;
-  fence_mbar_init();
   pdl_grid_dependency_wait();  // launched as a programmatic dependent: what is in front has completed from here on
   int run = 0, run_cost = 0;
   for (int b0 = 0; b0 < p.B; b0 += Cfg::NTHREADS) {
@@ -591,17 +585,23 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     }
     return lo;
   };
-  // units in front of a place in the order of costs; a head's own cost comes before its units
-  auto units_before = [&](int cost) {
-    if (cost >= total) return run * per_seq;
-    const int b = find(costs, cost);
-    const int n = pre[b + 1] - pre[b];
-    const int rem = cost - costs[b] * per_seq, item = kv_div(rem, n + kKvHeadCost);
-    const int in_head = rem - item * (n + kKvHeadCost);
-    return pre[b] * per_seq + item * n + (p.whole ? (in_head > 0 ? n : 0) : max(in_head - kKvHeadCost, 0));
+  // a place in the order of costs, where a head's own cost comes before its units: what it falls on, and the units in front of it
+  struct Place {
+    int b, n, item, in_head, units;
   };
-  const int t0 = units_before(range.first(blockIdx.x)), t1 = units_before(range.first(blockIdx.x + 1));
-  const int mine = t1 - t0;
+  auto place = [&](int cost) {
+    Place x;
+    x.b = find(costs, min(cost, total - 1));
+    x.n = pre[x.b + 1] - pre[x.b];
+    const int rem = min(cost, total - 1) - costs[x.b] * per_seq;
+    x.item = kv_div(rem, x.n + kKvHeadCost);
+    x.in_head = rem - x.item * (x.n + kKvHeadCost);
+    const int units = p.whole ? (x.in_head > 0 ? x.n : 0) : max(x.in_head - kKvHeadCost, 0);
+    x.units = cost < total ? pre[x.b] * per_seq + x.item * x.n + units : run * per_seq;
+    return x;
+  };
+  const Place begin = place(range.first(blockIdx.x)), end = place(range.first(blockIdx.x + 1));
+  const int t0 = begin.units, mine = end.units - t0;
   if (mine == 0) return;
 
   // a head's share of the run
@@ -609,27 +609,28 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     int b, head, n, from, to, row0, len;  // units [from, to) of n
     long long q_row0;
   };
-  auto part_at = [&](int at) {
+  auto part_of = [&](int b, int n, int item, int from, int left) {
     Part x;
-    const int b = x.b = find(pre, at);
-    x.n = pre[b + 1] - pre[b];
-    const int rem = at - pre[b] * per_seq, item = kv_div(rem, x.n), head = p.row_blocks == 1 ? item : item / p.row_blocks;
-    x.head = head;
-    x.from = rem - item * x.n;
-    x.to = min(x.n, x.from + (t1 - at));
-    x.row0 = (item - head * p.row_blocks) * ROWS;
+    x.b = b;
+    x.n = n;
+    x.head = p.row_blocks == 1 ? item : item / p.row_blocks;
+    x.from = from;
+    x.to = min(n, from + left);
+    x.row0 = (item - x.head * p.row_blocks) * ROWS;
     x.len = kv_length(p, b, false);
-    x.q_row0 = (static_cast<long long>(b) * p.cache.heads + head) * p.rows;
+    x.q_row0 = (static_cast<long long>(b) * p.cache.heads + x.head) * p.rows;
     return x;
   };
-  Part cur = part_at(t0);
+  auto part_at = [&](int done) {  // what comes after so many units of the run
+    const int at = t0 + done, b = find(pre, at), n = pre[b + 1] - pre[b], rem = at - pre[b] * per_seq, item = kv_div(rem, n);
+    return part_of(b, n, item, rem - item * n, mine - done);
+  };
+  Part cur = p.whole ? part_at(0) : part_of(begin.b, begin.n, begin.item, max(begin.in_head - kKvHeadCost, 0), mine);
   uint4 qx[Cfg::Q_PASSES];
   kv_load_q<Cfg>(qx, p, cur.q_row0, cur.row0);
 
   // ---------------------------------------------------------------------------------- fetching: unit k of this warp is t0 + warp + NW k
   uint8_t* ring = smem + warp * NSTAGE * Cfg::UNIT_BYTES;
-  uint64_t* full = bars + warp * NSTAGE;
-  int* gone = miss + warp * NSTAGE;
   const int nunits = mine > warp ? (mine - warp + NW - 1) / NW : 0;
   unsigned long long src0 = 0, src1 = 0;  // lane i: blocks of unit (k / 32) * 32 + i, 0: none there
   auto look_up = [&](int k0) {
@@ -657,34 +658,39 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
       }
     }
   };
-  int fetch_slot = 0;
-  auto fetch = [&](int k) {  // converged warp
-    if ((k & 31) == 0) look_up(k);
-    const unsigned long long a = __shfl_sync(0xffffffffu, src0, k & 31);
-    const unsigned long long b = Cfg::UNIT_BLOCKS > 1 ? __shfl_sync(0xffffffffu, src1, k & 31) : 0ull;
-    if (lane == 0) {
-      const int slot = fetch_slot;
-      uint8_t* to = ring + slot * Cfg::UNIT_BYTES;
-      gone[slot] = (a == 0 ? 1 : 0) | (Cfg::UNIT_BLOCKS > 1 && b == 0 ? 2 : 0);
-      mbar_expect_tx(&full[slot], ((a != 0) + (b != 0)) * Blk::BYTES);
-      if (a != 0 && b == a + Blk::BYTES) {
-        bulk_load_1d(to, reinterpret_cast<const void*>(a), 2 * Blk::BYTES, &full[slot]);
-      } else {
-        if (a != 0) bulk_load_1d(to, reinterpret_cast<const void*>(a), Blk::BYTES, &full[slot]);
-        if (b != 0) bulk_load_1d(to + Blk::BYTES, reinterpret_cast<const void*>(b), Blk::BYTES, &full[slot]);
+  // Every lane brings 16 bytes at a time; one group of copies per unit, empty ones behind the last.
+  int fetched = 0, missing = 0;  // missing: of the units in the ring, a bit for each block that is in no page
+  auto fetch = [&](int slot) {  // converged warp
+    if (fetched < nunits) {
+      if ((fetched & 31) == 0) look_up(fetched);
+      constexpr int FULL = Blk::BYTES / 512, REST = Blk::BYTES % 512 / 16;  // whole turns of the warp for a block, lanes of one more
+      unsigned long long a[2];
+      a[0] = __shfl_sync(0xffffffffu, src0, fetched & 31);
+      a[1] = Cfg::UNIT_BLOCKS > 1 ? __shfl_sync(0xffffffffu, src1, fetched & 31) : 0ull;
+      const uint32_t to = smem_u32(ring + slot * Cfg::UNIT_BYTES) + lane * 16;
+      missing &= ~(3 << (2 * slot));
+#pragma unroll
+      for (int i = 0; i < Cfg::UNIT_BLOCKS; ++i) {
+        if (a[i] == 0) {
+          missing |= 1 << (2 * slot + i);
+          continue;
+        }
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(a[i]) + lane * 16;
+#pragma unroll
+        for (int j = 0; j < FULL; ++j) kv_copy16(to + i * Blk::BYTES + j * 512, from + j * 512);
+        if (REST > 0 && lane < REST) kv_copy16(to + i * Blk::BYTES + FULL * 512, from + FULL * 512);
       }
+      ++fetched;
     }
-    fetch_slot = fetch_slot + 1 == NSTAGE ? 0 : fetch_slot + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int fetched = 0;
-  for (; fetched < nunits && fetched < NSTAGE; ++fetched) fetch(fetched);
-
+#pragma unroll
+  for (int i = 0; i < NSTAGE; ++i) fetch(i);
   kv_store_q<Cfg>(qx, qs, p, cur.row0, cur.len);
   __syncthreads();
 
   // ---------------------------------------------------------------------------------- the run, head by head
-  bool ok = true;
-  int k = 0, slot = 0, phase = 0;  // units of this warp that are done; where the next one is
+  int k = 0, slot = 0;  // units of this warp that are done; where the next one is
   KvAttnState<Cfg> st;
   st.vflip = (lane >> 2) & 1 ? static_cast<float>((1 << Cfg::BITS) - 1) : 0.f;
   for (int done = 0;;) {  // units of the run before this head
@@ -694,28 +700,25 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int kend = todo > warp ? (todo - warp + NW - 1) / NW : 0;
     int pos = (cur.from + warp + NW * k - done) * Cfg::UNIT;
     for (; k < kend; ++k, pos += NW * Cfg::UNIT) {
-      ok = ok && mbar_wait_warp(&full[slot], phase, ab, kTagKvFull);
-      if (!ok) break;
+      asm volatile("cp.async.wait_group %0;" ::"n"(NSTAGE - 1) : "memory");
+      __syncwarp();
       const uint8_t* blk = ring + slot * Cfg::UNIT_BYTES;
-      const int missing = gone[slot];
-      if (missing == 0 && pos + Cfg::UNIT <= clear) {
+      const int gone = (missing >> (2 * slot)) & 3;
+      if (gone == 0 && pos + Cfg::UNIT <= clear) {
         kv_attn_blocks<Cfg, Cfg::UNIT_BLOCKS, false>(st, blk, pos, cur.len, 0, lane);
       } else {
 #pragma unroll 1
         for (int i = 0; i < Cfg::UNIT_BLOCKS && pos + i * kKvBlockTokens < cur.len; ++i)
-          kv_attn_blocks<Cfg, 1, true>(st, blk + i * Blk::BYTES, pos + i * kKvBlockTokens, cur.len, (missing >> i) & 1, lane);
+          kv_attn_blocks<Cfg, 1, true>(st, blk + i * Blk::BYTES, pos + i * kKvBlockTokens, cur.len, (gone >> i) & 1, lane);
       }
-      __syncwarp();
-      if (fetched < nunits) fetch(fetched++);
-      if (++slot == NSTAGE) {
-        slot = 0;
-        phase ^= 1;
-      }
+      __syncwarp();  // every lane has read the slot
+      fetch(slot);
+      slot = slot + 1 == NSTAGE ? 0 : slot + 1;
     }
     const bool more = todo < mine;
     Part next;
     if (more) {
-      next = part_at(t0 + todo);
+      next = part_at(todo);
       kv_load_q<Cfg>(qx, p, next.q_row0, next.row0);
     }
 
@@ -794,10 +797,6 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     __syncthreads();
     cur = next;
     done = todo;
-  }
-  if (!ok) {  // abort path: what is on its way lands before this CTA's shared memory is released
-    if (lane == 0)
-      for (int i = max(0, fetched - NSTAGE); i < fetched; ++i) mbar_wait_drain(&full[i % NSTAGE], (i / NSTAGE) & 1, 2000000ull);
   }
 }
 
