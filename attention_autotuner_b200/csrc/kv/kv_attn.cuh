@@ -438,17 +438,19 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         if constexpr (Cfg::SPLIT) lo[r] = Kv16<false>::round2(wt[0] - Kv16<false>::lo(hi[r]), wt[1] - Kv16<false>::hi(hi[r]));
       }
       if constexpr (Cfg::HALF) {
-        hi[1] = own ? hi[0] : 0u;
-        hi[0] = own ? 0u : hi[0];
-        if constexpr (Cfg::SPLIT) {
-          lo[1] = own ? lo[0] : 0u;
-          lo[0] = own ? 0u : lo[0];
-        }
-      }
+        // Transposed, lanes of columns 0 to 3 have positions 0 to 7, those of columns 4 to 7 positions 8 to 15; the other places of
+        // the fragment take the second pieces, which columns 4 to 7 and 0 to 3 then hold: all columns of a row are added at the end.
+        const uint32_t x = kv_transpose8x8(hi[0]);
+        uint32_t rest = 0;
+        if constexpr (Cfg::SPLIT) rest = __shfl_xor_sync(0xffffffffu, kv_transpose8x8(lo[0]), 16);
+        pb[nb][nt][0] = lane < 16 ? x : rest;
+        pb[nb][nt][1] = lane < 16 ? rest : x;
+      } else {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        pb[nb][nt][r] = kv_transpose8x8(hi[r]);
-        if constexpr (Cfg::SPLIT) pl[nb][nt][r] = kv_transpose8x8(lo[r]);
+        for (int r = 0; r < 2; ++r) {
+          pb[nb][nt][r] = kv_transpose8x8(hi[r]);
+          if constexpr (Cfg::SPLIT) pl[nb][nt][r] = kv_transpose8x8(lo[r]);
+        }
       }
     }
   uint32_t w[NB][LANE_UNITS * 4];
@@ -485,7 +487,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         for (int nt = 0; nt < NT; ++nt) {
           float* acc = st.acc[TILES * x + i][nt];
           kv_mma(acc, f, pb[nb][nt], acc);
-          if constexpr (Cfg::SPLIT) kv_mma(acc, f, pl[nb][nt], acc);
+          if constexpr (Cfg::SPLIT && !Cfg::HALF) kv_mma(acc, f, pl[nb][nt], acc);
         }
       }
     }
