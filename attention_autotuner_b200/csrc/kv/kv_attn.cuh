@@ -71,8 +71,11 @@ struct KvAttnParams {
 };
 
 // Work: sequence b has n = units(b) of Cfg::UNIT positions for each (head, row block), and a head costs kKvHeadCost units more
-// (queries in, partial results out). The CTAs' runs are equal shares of that cost.
-constexpr int kKvHeadCost = 8;
+// (queries in, partial results out). The CTAs' runs are equal shares of that cost. Measured with 4 / 8 / 12 / 16 / 24 units: 64 sequences
+// of 100 to 4000 positions, 8 heads, d = 128, 4 bits 26.6 / 24.2 / 23.7 / 24.0 / 25.7 us (units of 32 positions); 32 of 64 to 4096,
+// four queries, 8 bits 34.3 / 30.3 / 26.6 / 24.6 / 25.2 (units of 16).
+template <int UNIT>
+constexpr int kKvHeadCost = UNIT == 32 ? 12 : 16;
 // a / b for quotients far below 2^22: the product with the reciprocal is off by less than one.
 __device__ __forceinline__ int kv_div(int a, int b) {
   const int q = static_cast<int>(__int2float_rn(a) * __frcp_rn(__int2float_rn(b))), r = a - q * b;
@@ -537,15 +540,15 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     for (int w = 0; w < NW; ++w) {
       if (w < warp) {
         before += scan[0][w];
-        before_cost += kKvHeadCost * scan[1][w];
+        before_cost += kKvHeadCost<Cfg::UNIT> * scan[1][w];
       }
       run += scan[0][w];
       heads += scan[1][w];
     }
-    run_cost += kKvHeadCost * heads + run;
+    run_cost += kKvHeadCost<Cfg::UNIT> * heads + run;
     if (b < p.B) {
       pre[b] = before + x - n;
-      costs[b] = before + x - n + before_cost + kKvHeadCost * __popc(some & ((1u << lane) - 1u));
+      costs[b] = before + x - n + before_cost + kKvHeadCost<Cfg::UNIT> * __popc(some & ((1u << lane) - 1u));
     }
     __syncthreads();
   }
@@ -596,9 +599,9 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     x.b = find(costs, min(cost, total - 1));
     x.n = pre[x.b + 1] - pre[x.b];
     const int rem = min(cost, total - 1) - costs[x.b] * per_seq;
-    x.item = kv_div(rem, x.n + kKvHeadCost);
-    x.in_head = rem - x.item * (x.n + kKvHeadCost);
-    const int units = p.whole ? (x.in_head > 0 ? x.n : 0) : max(x.in_head - kKvHeadCost, 0);
+    x.item = kv_div(rem, x.n + kKvHeadCost<Cfg::UNIT>);
+    x.in_head = rem - x.item * (x.n + kKvHeadCost<Cfg::UNIT>);
+    const int units = p.whole ? (x.in_head > 0 ? x.n : 0) : max(x.in_head - kKvHeadCost<Cfg::UNIT>, 0);
     x.units = cost < total ? pre[x.b] * per_seq + x.item * x.n + units : run * per_seq;
     return x;
   };
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int at = t0 + done, b = find(pre, at), n = pre[b + 1] - pre[b], rem = at - pre[b] * per_seq, item = kv_div(rem, n);
     return part_of(b, n, item, rem - item * n, mine - done);
   };
-  Part cur = p.whole ? part_at(0) : part_of(begin.b, begin.n, begin.item, max(begin.in_head - kKvHeadCost, 0), mine);
+  Part cur = p.whole ? part_at(0) : part_of(begin.b, begin.n, begin.item, max(begin.in_head - kKvHeadCost<Cfg::UNIT>, 0), mine);
   uint4 qx[Cfg::Q_PASSES];
   kv_load_q<Cfg>(qx, p, cur.q_row0, cur.row0);
 
@@ -827,8 +830,8 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
       heads_before += n > 0;
     }
   }
-  mine_before = __reduce_add_sync(0xffffffffu, mine_before + kKvHeadCost * heads_before);
-  mine_all = __reduce_add_sync(0xffffffffu, mine_all + kKvHeadCost * heads_all);
+  mine_before = __reduce_add_sync(0xffffffffu, mine_before + kKvHeadCost<UNIT> * heads_before);
+  mine_all = __reduce_add_sync(0xffffffffu, mine_all + kKvHeadCost<UNIT> * heads_all);
   if (lane == 0) {
     before[warp] = mine_before;
     all[warp] = mine_all;
@@ -843,10 +846,10 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
   int c0 = 0, c1 = 0;
   KvRange range{};
   if (n > 0) {
-    first = first * per_seq + item * (n + kKvHeadCost);  // in costs
+    first = first * per_seq + item * (n + kKvHeadCost<UNIT>);  // in costs
     range = kv_range(total * per_seq, grid, p.by_grid);
-    c0 = range.owner(first + kKvHeadCost);
-    c1 = range.owner(first + kKvHeadCost + n - 1);
+    c0 = range.owner(first + kKvHeadCost<UNIT>);
+    c1 = range.owner(first + kKvHeadCost<UNIT> + n - 1);
   }
   // nothing is read or written before the kernel in front has completed; every thread waits, so that this one completes after it
   pdl_grid_dependency_wait();
