@@ -515,8 +515,9 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
   const int lane = threadIdx.x & 31;
   const int per_seq = p.cache.heads * p.row_blocks;
 
-  pdl_launch_dependents();
   pdl_grid_dependency_wait();  // launched as a programmatic dependent: what is in front has completed from here on
+  // only now may the join kernel start, which reads the lengths before it waits for this one
+  pdl_launch_dependents();
   int run = 0, run_cost = 0;
   for (int b0 = 0; b0 < p.B; b0 += Cfg::NTHREADS) {
     const int b = b0 + threadIdx.x;
@@ -806,13 +807,15 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
 }
 
 // Adds the partial results of the heads that lie in more than one run, in the order of the runs. grid (B * heads * row blocks, GY): a
-// task is one row and 64 channels of it, and a block takes every GY-th. Up to 64 parts: a warp a task, eight loads of a lane in
-// flight. More (few heads make up the whole batch): the block turns the references of all parts into weights, then its warps add them.
+// task is one row and 64 channels of it, and a block takes every GY-th. Up to 64 parts (24 where a block has a single task): a warp a
+// task, eight loads of a lane in flight. More (few heads make up the whole batch): the block turns the references of all parts into
+// weights, then its warps add them.
 template <int D, int ROWS, int UNIT, bool BF16>
 __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant__ KvAttnParams p, int grid) {
   using T = Kv16<BF16>;
   constexpr int STRIDE = ROWS * (D + 2);
-  __shared__ float weight[kKvMaxRuns], red[2][16];
+  __shared__ float2 weight[kKvMaxRuns];  // of a part: reference, then weight; sum
+  __shared__ float red[2][16];
   __shared__ float2 so[16][32];
   __shared__ int before[16], all[16];
   const int NT = blockDim.x, NW = NT >> 5;
@@ -869,7 +872,7 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
   auto store_lse = [&](int row, float M, float L) {
     if (p.lse != nullptr) p.lse[out0 + row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
   };
-  if (parts <= 64) {
+  if (parts <= (gridDim.y >= tasks ? 24 : 64)) {
     for (int task = blockIdx.y + gridDim.y * warp; task < tasks; task += gridDim.y * NW) {
       const int row = task / PAIRS, pair = task % PAIRS;
       float m[2], l[2], M = -INFINITY, L = 0.f;
@@ -918,9 +921,9 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
     const int row = task / PAIRS, pair = task % PAIRS;
     float top = -INFINITY;
     for (int i = threadIdx.x; i < parts; i += NT) {
-      const float m = part_at(i)[ROWS * D + row];
-      weight[i] = m;  // its own weight, in a moment
-      top = fmaxf(top, m);
+      const float* at = part_at(i) + ROWS * D + row;
+      weight[i] = make_float2(at[0], at[ROWS]);  // its own, in a moment
+      top = fmaxf(top, weight[i].x);
     }
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
@@ -930,9 +933,10 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
     for (int w = 1; w < NW; ++w) M = fmaxf(M, red[0][w]);
     float sum = 0.f;
     for (int i = threadIdx.x; i < parts; i += NT) {
-      const float l = part_at(i)[ROWS * D + ROWS + row], w = kv_weight(weight[i], l, M);
-      weight[i] = w;
-      sum = fmaf(w, l, sum);
+      const float2 ml = weight[i];
+      const float w = kv_weight(ml.x, ml.y, M);
+      weight[i].x = w;
+      sum = fmaf(w, ml.y, sum);
     }
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
@@ -949,7 +953,7 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (i0 + j * NW < parts) {
-          const float w = weight[i0 + j * NW];
+          const float w = weight[i0 + j * NW].x;
           x.x = fmaf(w, y[j].x, x.x);
           x.y = fmaf(w, y[j].y, x.y);
         }

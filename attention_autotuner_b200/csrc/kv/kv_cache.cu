@@ -164,7 +164,7 @@ int kv_attn_launch(KvAttnParams p, size_t ws_bytes, cudaStream_t stream) {
   p.row_blocks = (p.rows + Cfg::ROWS - 1) / Cfg::ROWS;
   const long long items = static_cast<long long>(p.B) * p.cache.heads * p.row_blocks;
   const long long units = (static_cast<long long>(p.cache.table_width) << p.cache.page_shift) / Cfg::UNIT + 1 + kKvHeadCost<Cfg::UNIT>;
-  if (items > 0x7fffffff / units)
+  if (items > 0x7fffffff / units || static_cast<long long>(p.cache.heads) * p.row_blocks > 1 << 20)  // 32-bit numbers, kv_div
     return fail(kErrInvalidArgument, "kv_attn: %d sequences x %d heads x %d row blocks with tables of %d pages exceed 2^31 units of work", p.B,
                 p.cache.heads, p.row_blocks, p.cache.table_width);
   const int grid = kv_attn_grid<Cfg>(p.rows);

@@ -188,6 +188,7 @@ ATTN = [
     (1, 2, 4, 1, False, 16, (5000,)),
     (2, 1, 8, 2, True, 64, (9001, 33)),
     (1, 1, 1, 1, False, 128, (30000,)),
+    (19, 1, 16, 1, False, 64, (20, 0, 3) * 5 + (20000, 1, 2, 700)),
 ]
 
 
@@ -377,6 +378,22 @@ def test_captured_steps_see_new_tables_and_lengths():
     got = kv_cache_read(cache, table, start, None, 1)[0]
     assert torch.equal(got, held(new, 4).half())
     assert torch.equal(kv_cache_read(cache, table, i32(3, 3, 3, 3), None, 1)[0], hk[:, :, 3:4].half())  # as before the capture
+
+
+def test_lengths_that_the_kernel_before_wrote():
+    """Both kernels of a call see what the launch in front of it wrote, here for 200 calls without a pause."""
+    B, H, d = 3, 2, 64
+    start = i32(900, 0, 2000)
+    cache, table, k, v, g = filled(16, B, H, 2300, d, 4, 64, torch.float16, i32(2300, 2300, 2300))
+    q = torch.randn(B, 4 * H, 1, d, generator=g, device="cuda").half()
+    lengths, outs = start.clone(), []
+    for _ in range(200):
+        lengths.add_(1)
+        outs.append(kv_cache_attn(q, cache, table, lengths))
+    for i in (0, 1, 57, 199):
+        n = start + i + 1
+        check_attn(outs[i], attention64(q, k, v, n, False, 0.125)[1], *attention64(q, k, v, n, False, 0.125))
+        assert torch.equal(outs[i], kv_cache_attn(q, cache, table, n))
 
 
 def test_calls_on_another_stream_and_from_threads():
