@@ -4,23 +4,36 @@
 // The numbers kn, vn go into the tensor cores as they are; scales and zeros are applied in fp32, to a score and to a probability,
 // so that no value of the cache is ever rounded.
 //
-// What bounds it: reading the cache once, 136 bytes per position and head of K and V at 4 bits and d = 128. At the copy
-// bandwidth an SM takes in a block of 16 positions every 94 cycles, in which its four schedulers issue 376 instructions; a block costs
-// a warp about 220 (40 to unpack K, 48 to transpose and unpack V, 16 products, 16 additions, 50 for the softmax). So:
-//   * every warp works alone, on units of 16 or 32 positions that it fetches itself with one bulk copy each (two where a page has
-//     only half a unit) into a ring of its own: no warp waits for another until the last unit of a head is done;
+// What bounds it: reading the cache once, 136 bytes per position and head of K and V at 4 bits and d = 128. At the copy bandwidth
+// (6.55 TB/s) an SM takes in a block of 16 positions every 94 cycles, in which its four schedulers issue 376 instructions; a block
+// costs a warp about 240 (40 to unpack K, 64 to transpose and unpack V, 16 products, 50 for the softmax, the rest to fetch). So:
+//   * every warp works alone, on units of 16 or 32 positions that it fetches itself, 16 bytes a lane at a time, into a ring of its
+//     own: no warp waits for another until the last unit of a head is done;
 //   * S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 with positions, then channels, as the 16 rows: eight query rows fill the
 //     eight columns (a tcgen05 tile would pad them to 128), and the packed side is an A operand that a lane unpacks in
 //     registers, without shared memory in between: a nibble masked out of a word is an fp16 subnormal, n 2^-24 or n 2^-20, and
 //     goes into the product as that (1024 + n and an exact subtraction, the usual way, doubles the instructions);
+//   * with up to four rows the other four columns repeat them, and each lane takes half of its scores through the softmax;
 //   * the reference of the exponentials follows the running maximum only when a score is more than 2^4 above it, and so does the
 //     power of two by which the scales of V are brought into fp16 range; both are looked at with one vote per unit;
-//   * work is dealt out in equal runs of units over all CTAs, across heads and sequences of whatever lengths (the lengths are
-//     on the device, a captured launch sees new ones). A head that lies in one run is finished by its CTA; the others leave
+//   * work is dealt out in equal runs over all CTAs, across heads and sequences of whatever lengths (the lengths are on the
+//     device, a captured launch sees new ones). A head that lies in one run is finished by its CTA; the others leave
 //     maximum, sum and fp32 accumulator in scratch memory, and kv_attn_join_kernel, launched as a programmatic dependent, adds
 //     them in order. Nothing is added with atomics: the same call has the same bits.
-// With fp16 outputs a probability goes through the tensor cores in two pieces (its fp16 value and what that leaves), with bf16
-// in one: one piece alone is off by as much as rounding the output to fp16.
+// The accumulators of the tensor cores drop the bits that do not fit, always the same way, and run over a whole sequence. V of odd
+// positions counts from the other end (kv_format.cuh), so that both signs occur and the sums stay near zero: 131072 positions in
+// fp16 are 2.1e-4 from 64 bits, all of it the rounding of the output, where numbers from 0 were 7e-3 off. With fp16 outputs a
+// probability goes through the tensor cores in two pieces (its fp16 value and what that leaves), with bf16 in one: one piece
+// alone is off by as much as rounding the output to fp16.
+//
+// Measured (B200, us, calls one after another; at the copy bandwidth): 8 sequences of 131072 positions, 32 heads over 8, d = 128, 4 bits,
+// fp16 201 (174), 5.7 TB/s; 2 of 16384, 16 heads, 8 bits, bf16 28.5 (21); 32 of up to 8192, 32 over 8, 4 bits, bf16 22.2 (10.8); 16 of
+// up to 4096, four queries, 8 bits, fp16 14.7 (3.1); one of 50001, 8 heads over one, d = 256 14.4 (2.0); 2 of 512, 4 heads, d = 64 6.5.
+// What is left of the short ones: 3 us until the first unit has come (lengths, table, unit: three trips to memory behind one
+// another), 1 us to add the warps' results, 3 us for the second kernel; of the middle ones as well that SMs with the same share
+// of the bytes finish up to 25% apart. Tried and not kept: units by bulk copies and mbarriers (one lane's work holds up its warp:
+// 214 -> 220), three units in the ring (the SMs finish further apart, 28.6 -> 30.2 for 8 bits), four CTAs per SM (spills, 227),
+// CTAs of one or two warps (the partial results of more runs: 22.2 -> 24.4, 23.2), twice the runs (28.5 -> 35.2).
 #pragma once
 
 #include "../fast_div.cuh"
@@ -52,7 +65,7 @@ struct KvAttnConfig {
   static constexpr int STAT_BYTES = 3 * NWARPS * ROWS * 4;  // reference, sum, sum of p vz
   static constexpr int Q_BYTES = 8 * NT * (D * 2 + 16);  // fragments, and what kv_store_q says of a row
   static constexpr int Q_PASSES = (ROWS * D / 8 + NTHREADS - 1) / NTHREADS;
-  static constexpr int MIN_CTAS = NT * D <= 64 || ROWS * D <= 512 ? 3 : NT * D <= 128 ? 3 : 2;  // 128, 168 or 255 registers
+  static constexpr int MIN_CTAS = NT * D <= 128 ? 3 : 2;  // 168 or 255 registers
   static constexpr int part_bytes(int rows) { return NWARPS * (rows < ROWS ? rows : ROWS) * PART_STRIDE * 4; }
   static int smem_bytes(int rows, int B) { return RING_BYTES + Q_BYTES + STAT_BYTES + part_bytes(rows) + (B + 1) * 8; }
 };
