@@ -68,7 +68,7 @@ def attention64(q, k, v, lengths, causal, scale):
 
 def check_attn(o, lse, want, want_lse, weight):
     size, spread = weight[..., :-1], weight[..., -1:]
-    tol = torch.finfo(o.dtype).eps / 2 * want.abs() + 2.0 ** -14 * size + (2.0 ** -11 if o.dtype == torch.bfloat16 else 2.0 ** -22) * spread
+    tol = torch.finfo(o.dtype).eps / 2 * want.abs().clamp(min=torch.finfo(o.dtype).smallest_normal) + 2.0 ** -14 * size + (2.0 ** -11 if o.dtype == torch.bfloat16 else 2.0 ** -22) * spread
     bad = (o.double() - want).abs() > tol
     assert not bad.any(), ((o.double() - want).abs() / tol).max().item()
     none = want_lse == -math.inf
