@@ -15,7 +15,8 @@
 //     goes into the product as that (1024 + n and an exact subtraction, the usual way, doubles the instructions);
 //   * with up to four rows the other four columns repeat them, and each lane takes half of its scores through the softmax;
 //   * the reference of the exponentials follows the running maximum only when a score is more than 2^4 above it, and so does the
-//     power of two by which the scales of V are brought into fp16 range; both are looked at with one vote per unit;
+//     power of two by which a row's probabilities times scales of V are brought into fp16 range (of the products: a large value
+//     that has no weight, or none in this row, costs the others nothing); both are looked at with one vote per unit;
 //   * work is dealt out in equal runs over all CTAs, across heads and sequences of whatever lengths (the lengths are on the
 //     device, a captured launch sees new ones). A head that lies in one run is finished by its CTA; the others leave
 //     maximum, sum and fp32 accumulator in scratch memory, and kv_attn_join_kernel, launched as a programmatic dependent, adds
@@ -179,6 +180,9 @@ __device__ __forceinline__ float kv_weight(float m, float l, float M) {
   return ex2_approx(m - M);
 }
 
+// 1 / x of a power of two from 2^-126 to 2^126.
+__device__ __forceinline__ float kv_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 // The state of a warp for one (sequence, head, row block).
 template <class Cfg>
 struct KvAttnState {
@@ -189,8 +193,7 @@ struct KvAttnState {
   float m[NT][2], l[NT][2], z[NT][2];
   float acc[D / 16][NT][4];
   float vflip;                 // 0, or 2^bits - 1 for a lane whose positions are odd: their numbers of V are stored as that minus n
-  // scales of V are used times vup, a power of two and the sign of the lane's positions; they may reach vmax; vdown = 1 / |vup|
-  float vup, vdown, vmax;
+  float wup[NT][2];            // what brings a column's probabilities times scales of V into fp16: a power of two, minus at odd positions
 };
 
 // The query rows row0 ... of a head, a thread eight channels: fetched early, stored as the fragments of all warps.
@@ -275,6 +278,7 @@ __device__ __forceinline__ void kv_begin(KvAttnState<Cfg>& st, const uint8_t* qs
       st.lim[nt][i] = __float_as_int(r.z);
       st.m[nt][i] = -INFINITY;
       st.l[nt][i] = st.z[nt][i] = 0.f;
+      st.wup[nt][i] = st.vflip != 0.f ? -8.507059e37f : 8.507059e37f;  // 2^126: the first scale that is not zero brings it down
     }
   }
 #pragma unroll
@@ -283,7 +287,6 @@ __device__ __forceinline__ void kv_begin(KvAttnState<Cfg>& st, const uint8_t* qs
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) st.acc[u][nt][i] = 0.f;
-  st.vup = st.vdown = st.vmax = 0.f;
 }
 
 // NB blocks of 16 positions at blk, the first of them position pos0. EDGE: some of them are past the length or hidden from some
@@ -350,10 +353,18 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
       for (int i = 0; i < 2 * R; ++i) s[nb][nt][i] = Cfg::HALF && own ? sum[nt][i + 2] : sum[nt][i];
   }
 
-  // exponents against the present references
-  float e[NB][NT][2 * R];
+  // probabilities against the present references, and weights of the numbers of V
+  float e[NB][NT][2 * R], x[NB][NT][2 * R], wt[NB][NT][2 * R];
   bool hidden[NB][NT][2 * R];
-  auto exponents = [&] {
+  auto weights = [&] {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) wt[nb][nt][i] = EDGE && hidden[nb][nt][i] ? 0.f : x[nb][nt][i] * vs[nb][i >> 1] * st.wup[nt][i & 1];
+  };
+  auto probabilities = [&] {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -366,19 +377,22 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
             hidden[nb][nt][i] = ((missing >> nb) & 1) || pos0 + nb * 16 + g + own + 8 * r >= st.lim[nt][c];
             if (hidden[nb][nt][i]) e[nb][nt][i] = -INFINITY;
           }
+          x[nb][nt][i] = ex2_approx(e[nb][nt][i]);
         }
+    weights();
   };
-  exponents();
-  float vtop = 0.f, etop = -INFINITY;
+  probabilities();
+  float etop = -INFINITY, wtop = 0.f;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      vtop = fmaxf(vtop, vs[nb][r]);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) etop = fmax3(etop, e[nb][nt][2 * r], e[nb][nt][2 * r + 1]);
-    }
-  if (__any_sync(0xffffffffu, etop > 4.f || vtop > st.vmax)) {
+      for (int r = 0; r < R; ++r) {
+        etop = fmax3(etop, e[nb][nt][2 * r], e[nb][nt][2 * r + 1]);
+        wtop = fmax3(wtop, fabsf(wt[nb][nt][2 * r]), fabsf(wt[nb][nt][2 * r + 1]));
+      }
+  if (__any_sync(0xffffffffu, etop > 4.f || wtop > 16384.f)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -390,12 +404,12 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const int i = 2 * r + c;
-            float x = e[nb][nt][i] + st.m[nt][c];
+            float y = e[nb][nt][i] + st.m[nt][c];
             if (st.m[nt][c] == -INFINITY) {
-              x = fmaf(ks[nb][r] * st.cq[nt][c], s[nb][nt][i], kz[nb][r] * st.sq[nt][c]);
-              if (EDGE && hidden[nb][nt][i]) x = -INFINITY;
+              y = fmaf(ks[nb][r] * st.cq[nt][c], s[nb][nt][i], kz[nb][r] * st.sq[nt][c]);
+              if (EDGE && hidden[nb][nt][i]) y = -INFINITY;
             }
-            top = fmaxf(top, x);
+            top = fmaxf(top, y);
           }
         const float mn = fmaxf(st.m[nt][c], kv_max_rows<Cfg::HALF>(top));
         const float f = st.m[nt][c] == -INFINITY ? 0.f : ex2_approx(st.m[nt][c] - mn);
@@ -408,24 +422,31 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
           st.acc[u][nt][2 + c] *= f;
         }
       }
-    vtop = kv_max_rows<Cfg::HALF>(vtop);  // now the same in all lanes
-    if (vtop > st.vmax) {
-      // 2^x is the power of two above vtop; scales are used as multiples of 2^(x - 6): below 2^10 as long as they stay below
-      // 2^(x + 4), and below 2^14 with p below 2^4
-      const int x = max(static_cast<int>(__float_as_uint(vtop) >> 23) - 126, -120);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 6 - x) << 23);
-      const float f = up * st.vdown;
-      st.vmax = __uint_as_float(static_cast<uint32_t>(127 + min(x + 4, 127)) << 23);
-      st.vup = st.vflip != 0.f ? -up : up;
-      st.vdown = __uint_as_float(static_cast<uint32_t>(127 - 6 + x) << 23);
+    probabilities();
+    // columns with a weight above 2^14 get their largest one into [2^8, 2^9): what it is needed for is 2^-32 of that
 #pragma unroll
-      for (int u = 0; u < D / 16; ++u)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int c = 0; c < 2; ++c) {
+        float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) st.acc[u][nt][i] *= f;
-    }
-    exponents();
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (!EDGE || !hidden[nb][nt][2 * r + c]) top = fmaxf(top, x[nb][nt][2 * r + c] * vs[nb][r]);
+        top = kv_max_rows<Cfg::HALF>(top);
+        if (top * fabsf(st.wup[nt][c]) > 16384.f) {
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 + 127) - (__float_as_uint(top) >> 23) << 23);
+          const float f = up * kv_inverse(fabsf(st.wup[nt][c]));
+          st.wup[nt][c] = st.vflip != 0.f ? -up : up;
+#pragma unroll
+          for (int u = 0; u < D / 16; ++u) {
+            st.acc[u][nt][c] *= f;
+            st.acc[u][nt][2 + c] *= f;
+          }
+        }
+      }
+    weights();
   }
 
   uint32_t pb[NB][NT][2], pl[NB][NT][2];
@@ -436,31 +457,24 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
       uint32_t hi[2], lo[2];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float vscale = vs[nb][r] * st.vup;
-        float wt[2];
+        const float* w2 = &wt[nb][nt][2 * r];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int i = 2 * r + c;
-          const float x = ex2_approx(e[nb][nt][i]);
-          st.l[nt][c] += x;
-          if (!EDGE || !hidden[nb][nt][i]) {
-            st.z[nt][c] = fmaf(x, vz[nb][r], st.z[nt][c]);
-            wt[c] = x * vscale;
-          } else {
-            wt[c] = 0.f;
-          }
+          st.l[nt][c] += x[nb][nt][i];
+          if (!EDGE || !hidden[nb][nt][i]) st.z[nt][c] = fmaf(x[nb][nt][i], vz[nb][r], st.z[nt][c]);
         }
-        hi[r] = Kv16<false>::round2(wt[0], wt[1]);
-        if constexpr (Cfg::SPLIT) lo[r] = Kv16<false>::round2(wt[0] - Kv16<false>::lo(hi[r]), wt[1] - Kv16<false>::hi(hi[r]));
+        hi[r] = Kv16<false>::round2(w2[0], w2[1]);
+        if constexpr (Cfg::SPLIT) lo[r] = Kv16<false>::round2(w2[0] - Kv16<false>::lo(hi[r]), w2[1] - Kv16<false>::hi(hi[r]));
       }
       if constexpr (Cfg::HALF) {
         // Transposed, lanes of columns 0 to 3 have positions 0 to 7, those of columns 4 to 7 positions 8 to 15; the other places of
         // the fragment take the second pieces, which columns 4 to 7 and 0 to 3 then hold: all columns of a row are added at the end.
-        const uint32_t x = kv_transpose8x8(hi[0]);
+        const uint32_t most = kv_transpose8x8(hi[0]);
         uint32_t rest = 0;
         if constexpr (Cfg::SPLIT) rest = __shfl_xor_sync(0xffffffffu, kv_transpose8x8(lo[0]), 16);
-        pb[nb][nt][0] = lane < 16 ? x : rest;
-        pb[nb][nt][1] = lane < 16 ? rest : x;
+        pb[nb][nt][0] = lane < 16 ? most : rest;
+        pb[nb][nt][1] = lane < 16 ? rest : most;
       } else {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -477,11 +491,11 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
       *reinterpret_cast<uint4*>(w[nb] + 4 * u) = *reinterpret_cast<const uint4*>(blk + nb * Blk::BYTES + Blk::CODE + (u * 32 + lane) * 16);
   constexpr int TILES = BITS == 4 ? 4 : 2;  // of 16 channels in a word of each of eight lanes
 #pragma unroll
-  for (int x = 0; x < VW; ++x) {
+  for (int v = 0; v < VW; ++v) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       // positions 2t, 2t + 1 | 2t + 8, 2t + 9: their halves side by side, then pairs of one channel
-      const uint32_t a = w[nb][x], b = w[nb][VW + x], c = w[nb][2 * VW + x], d = w[nb][3 * VW + x];
+      const uint32_t a = w[nb][v], b = w[nb][VW + v], c = w[nb][2 * VW + v], d = w[nb][3 * VW + v];
       uint32_t ab[2] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632)};
       uint32_t cd[2] = {__byte_perm(c, d, 0x5410), __byte_perm(c, d, 0x7632)};
 #pragma unroll
@@ -501,7 +515,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float* acc = st.acc[TILES * x + i][nt];
+          float* acc = st.acc[TILES * v + i][nt];
           kv_mma(acc, f, pb[nb][nt], acc);
           if constexpr (Cfg::SPLIT && !Cfg::HALF) kv_mma(acc, f, pl[nb][nt], acc);
         }
@@ -745,13 +759,14 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int g = lane >> 2, t = lane & 3;
     const int nrows = min(ROWS, p.rows - cur.row0);
     // what the numbers were taken for: odd channels of 4 bits times 16
-    const float even = st.vdown * (Cfg::BITS == 4 && Cfg::SPLIT ? 16384.f : kKvLoUnit), odd = st.vdown * (Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit);
+    constexpr float EVEN = Cfg::BITS == 4 && Cfg::SPLIT ? 16384.f : kKvLoUnit, ODD = Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float l = kv_sum_rows<Cfg::HALF>(st.l[nt][c]), z = kv_sum_rows<Cfg::HALF>(st.z[nt][c]);
         const int row = nt * 8 + 2 * t + c;
+        const float down = kv_inverse(fabsf(st.wup[nt][c])), even = down * EVEN, odd = down * ODD;
         if constexpr (Cfg::HALF) {
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) {

@@ -244,6 +244,26 @@ def test_growing_peaks_and_scales(bits, name):
         check_attn(o, lse, want, want_lse, weight)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("group", [2, 8])
+def test_large_values_without_weight(bits, group):
+    """Values 2^40 times the others in a place that one of two queries does not see, and where the probability is 2^-60: what is
+    left of the row is as exact as without them."""
+    d, L = 64, 300
+    k, v, g = make(17, 1, 1, L, d, torch.bfloat16)
+    q = torch.randn(1, group, 2, d, generator=g, device="cuda").bfloat16()
+    v[:, :, L - 1] *= 2.0 ** 40                                     # the last position: query 0 does not see it
+    k[:, :, 100] = (-30 * q[0, 0, 0] / q[0, 0, 0].float().norm()).bfloat16()  # query 0 of head 0: a score far below the others
+    v[:, :, 100] *= 2.0 ** 40
+    cache = QuantizedKVCache(5, 1, d, bits=bits, page_size=64, dtype=torch.bfloat16)
+    table = i32(3, 1, 4, 0, 2).reshape(1, 5)
+    kv_cache_write(cache, k, v, table, i32(0))
+    o, lse = kv_cache_attn(q, cache, table, i32(L), None, True, 1.0, True)
+    want, want_lse, weight = attention64(q, held(k, bits), held(v, bits), i32(L), True, 1.0)
+    check_attn(o[:, :1, :1], lse[:, :1, :1], want[:, :1, :1], want_lse[:, :1, :1], weight[:, :1, :1])
+    check_attn(o, lse, want, want_lse, weight)
+
+
 def test_values_beyond_the_range_of_fp16():
     """bf16 keys, values and queries of 2^-60 and 2^60: scales and zeros are applied in fp32."""
     for up in (-60, 60):
