@@ -356,14 +356,6 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
   // probabilities against the present references, and weights of the numbers of V
   float e[NB][NT][2 * R], x[NB][NT][2 * R], wt[NB][NT][2 * R];
   bool hidden[NB][NT][2 * R];
-  auto weights = [&] {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2 * R; ++i) wt[nb][nt][i] = EDGE && hidden[nb][nt][i] ? 0.f : x[nb][nt][i] * vs[nb][i >> 1] * st.wup[nt][i & 1];
-  };
   auto probabilities = [&] {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -378,8 +370,8 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
             if (hidden[nb][nt][i]) e[nb][nt][i] = -INFINITY;
           }
           x[nb][nt][i] = ex2_approx(e[nb][nt][i]);
+          wt[nb][nt][i] = EDGE && hidden[nb][nt][i] ? 0.f : x[nb][nt][i] * vs[nb][r] * st.wup[nt][c];
         }
-    weights();
   };
   probabilities();
   float etop = -INFINITY, wtop = 0.f;
@@ -393,29 +385,35 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         wtop = fmax3(wtop, fabsf(wt[nb][nt][2 * r]), fabsf(wt[nb][nt][2 * r + 1]));
       }
   if (__any_sync(0xffffffffu, etop > 4.f || wtop > 16384.f)) {
+    // per column: the largest score, and the largest score plus logarithm of a scale of V, from the scores themselves
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = -INFINITY;
-        // e is against m: infinite while there is no reference, so the first one is taken from the scores themselves
+        float top = -INFINITY, wide = -INFINITY;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const int i = 2 * r + c;
-            float y = e[nb][nt][i] + st.m[nt][c];
-            if (st.m[nt][c] == -INFINITY) {
-              y = fmaf(ks[nb][r] * st.cq[nt][c], s[nb][nt][i], kz[nb][r] * st.sq[nt][c]);
-              if (EDGE && hidden[nb][nt][i]) y = -INFINITY;
-            }
+            if (EDGE && hidden[nb][nt][i]) continue;
+            const float y = fmaf(ks[nb][r] * st.cq[nt][c], s[nb][nt][i], kz[nb][r] * st.sq[nt][c]);
             top = fmaxf(top, y);
+            wide = fmaxf(wide, y + __log2f(vs[nb][r]));
           }
         const float mn = fmaxf(st.m[nt][c], kv_max_rows<Cfg::HALF>(top));
-        const float f = st.m[nt][c] == -INFINITY ? 0.f : ex2_approx(st.m[nt][c] - mn);
+        wide = kv_max_rows<Cfg::HALF>(wide) - mn;  // of the largest weight
+        float f = st.m[nt][c] == -INFINITY ? 0.f : ex2_approx(st.m[nt][c] - mn);
         st.m[nt][c] = mn;
         st.l[nt][c] *= f;
         st.z[nt][c] *= f;
+        // a weight above 2^14 is brought to 2^8 or just below it: what it is needed for reaches 2^-32 of that
+        const float was = fabsf(st.wup[nt][c]);
+        if (wide > 14.f - static_cast<float>(static_cast<int>(__float_as_uint(was) >> 23) - 127)) {
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - static_cast<int>(ceilf(wide))) << 23);
+          f *= up * kv_inverse(was);
+          st.wup[nt][c] = st.vflip != 0.f ? -up : up;
+        }
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) {
           st.acc[u][nt][c] *= f;
@@ -423,30 +421,6 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         }
       }
     probabilities();
-    // columns with a weight above 2^14 get their largest one into [2^8, 2^9): what it is needed for is 2^-32 of that
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float top = 0.f;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (!EDGE || !hidden[nb][nt][2 * r + c]) top = fmaxf(top, x[nb][nt][2 * r + c] * vs[nb][r]);
-        top = kv_max_rows<Cfg::HALF>(top);
-        if (top * fabsf(st.wup[nt][c]) > 16384.f) {
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 + 127) - (__float_as_uint(top) >> 23) << 23);
-          const float f = up * kv_inverse(fabsf(st.wup[nt][c]));
-          st.wup[nt][c] = st.vflip != 0.f ? -up : up;
-#pragma unroll
-          for (int u = 0; u < D / 16; ++u) {
-            st.acc[u][nt][c] *= f;
-            st.acc[u][nt][2 + c] *= f;
-          }
-        }
-      }
-    weights();
   }
 
   uint32_t pb[NB][NT][2], pl[NB][NT][2];
