@@ -6,7 +6,7 @@
 //
 // What bounds it: reading the cache once, 136 bytes per position and head of K and V at 4 bits and d = 128. At the copy bandwidth
 // (6.55 TB/s) an SM takes in a block of 16 positions every 94 cycles, in which its four schedulers issue 376 instructions; a block
-// costs a warp about 240 (40 to unpack K, 64 to transpose and unpack V, 16 products, 50 for the softmax, the rest to fetch). So:
+// costs a warp about 245 (40 to unpack K, 64 to transpose and unpack V, 16 products, 50 for the softmax, the rest to fetch). So:
 //   * every warp works alone, on units of 16 or 32 positions that it fetches itself, 16 bytes a lane at a time, into a ring of its
 //     own: no warp waits for another until the last unit of a head is done;
 //   * S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 with positions, then channels, as the 16 rows: eight query rows fill the
@@ -28,8 +28,8 @@
 // alone is off by as much as rounding the output to fp16.
 //
 // Measured (B200, us, calls one after another; at the copy bandwidth): 8 sequences of 131072 positions, 32 heads over 8, d = 128, 4 bits,
-// fp16 201 (174), 5.7 TB/s; 2 of 16384, 16 heads, 8 bits, bf16 28.5 (21); 32 of up to 8192, 32 over 8, 4 bits, bf16 22.2 (10.8); 16 of
-// up to 4096, four queries, 8 bits, fp16 14.7 (3.1); one of 50001, 8 heads over one, d = 256 14.4 (2.0); 2 of 512, 4 heads, d = 64 6.5.
+// fp16 200 (174), 5.7 TB/s; 2 of 16384, 16 heads, 8 bits, bf16 28.4 (21); 32 of up to 8192, 32 over 8, 4 bits, bf16 22.5 (10.8); 16 of
+// up to 4096, four queries, 8 bits, fp16 15.0 (3.1); one of 50001, 8 heads over one, d = 256 14.4 (2.0); 2 of 512, 4 heads, d = 64 6.5.
 // What is left of the short ones: 3 us until the first unit has come (lengths, table, unit: three trips to memory behind one
 // another), 1 us to add the warps' results, 3 us for the second kernel; of the middle ones as well that SMs with the same share
 // of the bytes finish up to 25% apart. Tried and not kept: units by bulk copies and mbarriers (one lane's work holds up its warp:
