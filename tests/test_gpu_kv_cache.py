@@ -400,6 +400,47 @@ def test_captured_steps_see_new_tables_and_lengths():
     assert torch.equal(kv_cache_read(cache, table, i32(3, 3, 3, 3), None, 1)[0], hk[:, :, 3:4].half())  # as before the capture
 
 
+def test_a_captured_step_behind_copies_and_another_stream():
+    """What stands in front of the cache's kernels in a graph may be a copy, a fill, or the join of two streams."""
+    B, H, d = 2, 2, 128
+    cache, table, k, v, g = filled(18, B, H, 200, d, 4, 64, torch.float16, i32(200, 150))
+    q_in, new_in = (torch.randn(B, n, 1, d, generator=g, device="cuda").half() for n in (8, 2))
+    q, new, lengths = torch.empty_like(q_in), torch.empty_like(new_in), i32(0, 0)
+    host = torch.tensor([200, 150], dtype=torch.int32).pin_memory()
+    side, main = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def step():
+        lengths.copy_(host, non_blocking=True)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            new.copy_(new_in)
+            torch.mul(q_in, 0.5, out=q)
+        main.wait_stream(side)
+        kv_cache_write(cache, new, new, table, lengths - 1)
+        return kv_cache_attn(q, cache, table, lengths)
+
+    with torch.cuda.stream(main):
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            o = step()
+    for n in ((200, 150), (180, 2), (1, 199)):
+        host.copy_(torch.tensor(n, dtype=torch.int32))
+        new_in.normal_(generator=g)
+        q_in.normal_(generator=g)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(main):
+            graph.replay()
+        torch.cuda.synchronize()
+        for b in range(B):
+            k[b, :, n[b] - 1] = held(new_in[b, :, 0], 4)
+            v[b, :, n[b] - 1] = held(new_in[b, :, 0], 4)
+        want = attention64(q_in * 0.5, k, v, lengths, False, 0.125)
+        keep = torch.tensor([x <= (200, 150)[b] for b, x in enumerate(n)], device="cuda")  # positions behind 150 of sequence 1 were not written
+        check_attn(o[keep], want[1][keep], *(x[keep] for x in want))
+
+
 def test_lengths_that_the_kernel_before_wrote():
     """Both kernels of a call see what the launch in front of it wrote, here for 200 calls without a pause."""
     B, H, d = 3, 2, 64
