@@ -14,9 +14,10 @@
 //     registers, without shared memory in between: a nibble masked out of a word is an fp16 subnormal, n 2^-24 or n 2^-20, and
 //     goes into the product as that (1024 + n and an exact subtraction, the usual way, doubles the instructions);
 //   * with up to four rows the other four columns repeat them, and each lane takes half of its scores through the softmax;
-//   * the reference of the exponentials follows the running maximum only when a score is more than 2^4 above it, and so does the
-//     power of two by which a row's probabilities times scales of V are brought into fp16 range (of the products: a large value
-//     that has no weight, or none in this row, costs the others nothing); both are looked at with one vote per unit;
+//   * the reference of the exponentials follows the running maximum only when a score is more than 2^4 above it, and the power of
+//     two by which a row's probabilities times scales of V are brought into fp16 range falls when one of them leaves it and rises
+//     with the reference (of the products: a large value that has no weight, none any more, or none in this row, costs the others
+//     nothing); both are looked at with one vote per unit;
 //   * work is dealt out in equal runs over all CTAs, across heads and sequences of whatever lengths (the lengths are on the
 //     device, a captured launch sees new ones). A head that lies in one run is finished by its CTA; the others leave
 //     maximum, sum and fp32 accumulator in scratch memory, and kv_attn_join_kernel, launched as a programmatic dependent, adds
@@ -401,23 +402,25 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
             top = fmaxf(top, y);
             wide = fmaxf(wide, y + __log2f(vs[nb][r]));
           }
-        const float mn = fmaxf(st.m[nt][c], kv_max_rows<Cfg::HALF>(top));
+        // The reference is a whole number, so that what it moves by is taken out of the sums exactly.
+        const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)));
         wide = kv_max_rows<Cfg::HALF>(wide) - mn;  // of the largest weight
-        float f = st.m[nt][c] == -INFINITY ? 0.f : ex2_approx(st.m[nt][c] - mn);
+        const uint32_t fe = __float2uint_rz(127.f - (mn - st.m[nt][c]));  // 0 beyond 2^127, from -inf, and where nothing was seen yet
+        const float f = __uint_as_float(fe << 23);
         st.m[nt][c] = mn;
         st.l[nt][c] *= f;
         st.z[nt][c] *= f;
-        // a weight above 2^14 is brought to 2^8 or just below it: what it is needed for reaches 2^-32 of that
+        // What was added before has lost 1 / f of its weight, and the range of the weights may rise by as much. A weight above 2^8
+        // is brought there or just below it: what it is needed for reaches 2^-32 of that, and the next ones have room to grow.
         const float was = fabsf(st.wup[nt][c]);
-        if (wide > 14.f - static_cast<float>(static_cast<int>(__float_as_uint(was) >> 23) - 127)) {
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - static_cast<int>(ceilf(wide))) << 23);
-          f *= up * kv_inverse(was);
-          st.wup[nt][c] = st.vflip != 0.f ? -up : up;
-        }
+        const int risen = min(static_cast<int>((__float_as_uint(was) >> 23) + 127u - fe), 253);
+        const uint32_t up = static_cast<uint32_t>(min(risen, 135 - static_cast<int>(ceilf(fmaxf(wide, -200.f))))) << 23;
+        st.wup[nt][c] = st.vflip != 0.f ? -__uint_as_float(up) : __uint_as_float(up);
+        const float g2 = f * __uint_as_float(up) * kv_inverse(was);
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) {
-          st.acc[u][nt][c] *= f;
-          st.acc[u][nt][2 + c] *= f;
+          st.acc[u][nt][c] *= g2;
+          st.acc[u][nt][2 + c] *= g2;
         }
       }
     probabilities();
