@@ -181,6 +181,10 @@ __device__ __forceinline__ float kv_weight(float m, float l, float M) {
   return ex2_approx(m - M);
 }
 
+// The reference lies this much above the largest score (in exp2 units): the sums of a row, not yet divided, then stay below 2^-20 times
+// positions times the largest value, in fp32 for every finite bf16 value up to a million positions. What lies 2^102 below the largest
+// probability is lost for it, and scales of V lose bits below 2^-94.
+constexpr float kKvBelow = 24.f;
 // 1 / x of a power of two from 2^-126 to 2^126.
 __device__ __forceinline__ float kv_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
@@ -385,7 +389,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         etop = fmax3(etop, e[nb][nt][2 * r], e[nb][nt][2 * r + 1]);
         wtop = fmax3(wtop, fabsf(wt[nb][nt][2 * r]), fabsf(wt[nb][nt][2 * r + 1]));
       }
-  if (__any_sync(0xffffffffu, etop > 4.f || wtop > 16384.f)) {
+  if (__any_sync(0xffffffffu, etop > 4.f - kKvBelow || wtop > 16384.f)) {
     // per column: the largest score, and the largest score plus logarithm of a scale of V, from the scores themselves
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -403,17 +407,17 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
             wide = fmaxf(wide, y + __log2f(vs[nb][r]));
           }
         // The reference is a whole number, so that what it moves by is taken out of the sums exactly.
-        const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)));
+        const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)) + kKvBelow);
         wide = kv_max_rows<Cfg::HALF>(wide) - mn;  // of the largest weight
-        const uint32_t fe = __float2uint_rz(127.f - (mn - st.m[nt][c]));  // 0 beyond 2^127, from -inf, and where nothing was seen yet
-        const float f = __uint_as_float(fe << 23);
+        const int drop = static_cast<int>(fminf(mn - st.m[nt][c], 252.f));  // 252 from -inf too, and where nothing was seen yet
+        const float f = __uint_as_float(static_cast<uint32_t>(max(127 - drop, 0)) << 23);
         st.m[nt][c] = mn;
         st.l[nt][c] *= f;
         st.z[nt][c] *= f;
         // What was added before has lost 1 / f of its weight, and the range of the weights may rise by as much. A weight above 2^8
         // is brought there or just below it: what it is needed for reaches 2^-32 of that, and the next ones have room to grow.
         const float was = fabsf(st.wup[nt][c]);
-        const int risen = min(static_cast<int>((__float_as_uint(was) >> 23) + 127u - fe), 253);
+        const int risen = min(static_cast<int>(__float_as_uint(was) >> 23) + drop, 253);
         const uint32_t up = static_cast<uint32_t>(min(risen, 135 - static_cast<int>(ceilf(fmaxf(wide, -200.f))))) << 23;
         st.wup[nt][c] = st.vflip != 0.f ? -__uint_as_float(up) : __uint_as_float(up);
         const float g2 = f * __uint_as_float(up) * kv_inverse(was);
@@ -743,7 +747,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
       for (int c = 0; c < 2; ++c) {
         const float l = kv_sum_rows<Cfg::HALF>(st.l[nt][c]), z = kv_sum_rows<Cfg::HALF>(st.z[nt][c]);
         const int row = nt * 8 + 2 * t + c;
-        const float down = kv_inverse(fabsf(st.wup[nt][c])), even = down * EVEN, odd = down * ODD;
+        const float down = kv_inverse(fabsf(st.wup[nt][c]));  // a factor of its own: with EVEN or ODD it may exceed fp32
         if constexpr (Cfg::HALF) {
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) {
@@ -760,8 +764,8 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
           float* dst = part + (warp * part_rows + row) * PS + g * (D / 8);
 #pragma unroll
           for (int u = 0; u < D / 16; u += 2)
-            *reinterpret_cast<float4*>(dst + 2 * u) = make_float4(st.acc[u][nt][c] * even, st.acc[u][nt][2 + c] * odd,
-                                                                  st.acc[u + 1][nt][c] * even, st.acc[u + 1][nt][2 + c] * odd);
+            *reinterpret_cast<float4*>(dst + 2 * u) = make_float4(st.acc[u][nt][c] * EVEN * down, st.acc[u][nt][2 + c] * ODD * down,
+                                                                  st.acc[u + 1][nt][c] * EVEN * down, st.acc[u + 1][nt][2 + c] * ODD * down);
         }
       }
     __syncthreads();

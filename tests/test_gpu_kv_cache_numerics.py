@@ -46,3 +46,33 @@ def test_scores_rise_while_values_fall(bits, name, group, shape):
             cache, table = one_sequence(kk, vv, bits, 64, g)
             o, lse = kv_cache_attn(q, cache, table, i32(L), None, False, 1.0, True)
             check_attn(o, lse, *attention64(q, held(kk, bits), held(vv, bits), i32(L), False, 1.0))
+
+
+@pytest.mark.parametrize("group", [2, 8, 16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_values_near_the_largest_of_bf16(bits, group):
+    """Finite values whose weighted mean is finite: a few of 1e36, many of up to 3e38 (whose sum is not), rows of one value, and one of 1e36
+    that comes first and has lost its weight, among values of 1e-20."""
+    d = 64
+    g = torch.Generator("cuda").manual_seed(50)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+
+    towards = normal(d)
+    for L, make in ((5, lambda: normal(5, d) * 1e36), (3000, lambda: 1e38 * (1 + 2 * torch.rand(3000, d, generator=g, device="cuda"))),
+                    (400, lambda: torch.full((400, d), 3e38, device="cuda")), (512, None), (6000, None)):
+        k = 0.1 * normal(L, d)
+        if make is None:
+            v = normal(L, d) * 1e-20
+            v[0] = normal(d) * 1e36
+            k[:32] -= 200 * towards / towards.norm() ** 2  # 2^-288 of the others' probability
+        else:
+            v = make()
+        q = (towards + 0.05 * normal(1, group, 1, d)).bfloat16()
+        k, v = k.bfloat16()[None, None], v.bfloat16()[None, None]
+        cache, table = one_sequence(k, v, bits, 64, g)
+        o, lse = kv_cache_attn(q, cache, table, i32(L), None, False, 1.0, True)
+        want, want_lse, weight = attention64(q, held(k, bits), held(v, bits), i32(L), False, 1.0)
+        assert o.isfinite().all()
+        check_attn(o, lse, want, want_lse, weight)
