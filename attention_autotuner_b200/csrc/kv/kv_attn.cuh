@@ -22,9 +22,10 @@
 //     device, a captured launch sees new ones). A head that lies in one run is finished by its CTA; the others leave
 //     maximum, sum and fp32 accumulator in scratch memory, and kv_attn_join_kernel, launched as a programmatic dependent, adds
 //     them in order. Nothing is added with atomics: the same call has the same bits.
-// The accumulators of the tensor cores drop the bits that do not fit, always the same way, and run over a whole sequence. V of odd
-// positions counts from the other end (kv_format.cuh), so that both signs occur and the sums stay near zero: 131072 positions in
-// fp16 are 2.1e-4 from 64 bits, all of it the rounding of the output, where numbers from 0 were 7e-3 off. With fp16 outputs a
+// The accumulators of the tensor cores drop the bits that do not fit, always the same way. V of odd positions counts from the other end
+// (kv_format.cuh), so that both signs occur and the sums stay near zero where a channel's values lie about the middle of their rows'
+// ranges: 131072 positions in fp16 are then 2.1e-4 from 64 bits, all of it the rounding of the output, where numbers from 0 were 7e-3
+// off. For values at one end of the range, accumulators run over 1024 positions of a warp (HELD) and not over a sequence. With fp16 outputs a
 // probability goes through the tensor cores in two pieces (its fp16 value and what that leaves), with bf16 in one: one piece
 // alone is off by as much as rounding the output to fp16.
 //
@@ -62,6 +63,11 @@ struct KvAttnConfig {
   static constexpr int UNIT = UNIT_BLOCKS * kKvBlockTokens;       // positions
   static constexpr int UNIT_BYTES = UNIT_BLOCKS * Blk::BYTES;
   static constexpr int NSTAGE = UNIT_BYTES <= 2304 ? 4 : 2;
+  // Units of a warp until its accumulators are added to fp32 sums in shared memory and begin anew. The tensor cores drop the bits that
+  // do not fit, always the same way. A channel of V 40 above the others, which puts those at one end of their numbers, 65536 positions
+  // in one CTA, fp16: up to 4.6e-4 of sum p |v| beyond the rounding of the output, after 1024 positions 6.1e-5, after 512 3.5e-5;
+  // 8 of 131072 take 202, 205 and 208 us.
+  static constexpr int HELD = 1024 / UNIT;
   static constexpr int RING_BYTES = NWARPS * NSTAGE * UNIT_BYTES;
   static constexpr int PART_STRIDE = D + 4;  // floats of a row: the rows of a warp's store fall on other banks
   static constexpr int STAT_BYTES = 3 * NWARPS * ROWS * 4;  // reference, sum, sum of p vz
@@ -185,6 +191,10 @@ __device__ __forceinline__ float kv_weight(float m, float l, float M) {
 // positions times the largest value, in fp32 for every finite bf16 value up to a million positions. What lies 2^102 below the largest
 // probability is lost for it, and scales of V lose bits below 2^-94.
 constexpr float kKvBelow = 24.f;
+// 2^-x of a whole number x from 0; 0 beyond 126, and of NaN (from -inf to -inf).
+__device__ __forceinline__ float kv_fall(float x) {
+  return __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(fminf(x, 127.f))) << 23);
+}
 // 1 / x of a power of two from 2^-126 to 2^126.
 __device__ __forceinline__ float kv_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
@@ -286,12 +296,6 @@ __device__ __forceinline__ void kv_begin(KvAttnState<Cfg>& st, const uint8_t* qs
       st.wup[nt][i] = st.vflip != 0.f ? -8.507059e37f : 8.507059e37f;  // 2^126: the first scale that is not zero brings it down
     }
   }
-#pragma unroll
-  for (int u = 0; u < D / 16; ++u)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.acc[u][nt][i] = 0.f;
 }
 
 // NB blocks of 16 positions at blk, the first of them position pos0. EDGE: some of them are past the length or hidden from some
@@ -410,7 +414,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)) + kKvBelow);
         wide = kv_max_rows<Cfg::HALF>(wide) - mn;  // of the largest weight
         const int drop = static_cast<int>(fminf(mn - st.m[nt][c], 252.f));  // 252 from -inf too, and where nothing was seen yet
-        const float f = __uint_as_float(static_cast<uint32_t>(max(127 - drop, 0)) << 23);
+        const float f = kv_fall(mn - st.m[nt][c]);
         st.m[nt][c] = mn;
         st.l[nt][c] *= f;
         st.z[nt][c] *= f;
@@ -713,21 +717,71 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int todo = done + (cur.to - cur.from);
     const int kend = todo > warp ? (todo - warp + NW - 1) / NW : 0;
     int pos = (cur.from + warp + NW * k - done) * Cfg::UNIT;
-    for (; k < kend; ++k, pos += NW * Cfg::UNIT) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(NSTAGE - 1) : "memory");
-      __syncwarp();
-      const uint8_t* blk = ring + slot * Cfg::UNIT_BYTES;
-      const int gone = (missing >> (2 * slot)) & 3;
-      if (gone == 0 && pos + Cfg::UNIT <= clear) {
-        kv_attn_blocks<Cfg, Cfg::UNIT_BLOCKS, false>(st, blk, pos, cur.len, 0, lane);
-      } else {
+    const int g = lane >> 2, t = lane & 3;
+    const int nrows = min(ROWS, p.rows - cur.row0);
+    // what the numbers were taken for: odd channels of 4 bits times 16
+    constexpr float EVEN = Cfg::BITS == 4 && Cfg::SPLIT ? 16384.f : kKvLoUnit, ODD = Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit;
+    for (bool first = true;; first = false) {
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.acc[u][nt][i] = 0.f;
+      for (const int kstop = min(kend, k + Cfg::HELD); k < kstop; ++k, pos += NW * Cfg::UNIT) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(NSTAGE - 1) : "memory");
+        __syncwarp();
+        const uint8_t* blk = ring + slot * Cfg::UNIT_BYTES;
+        const int gone = (missing >> (2 * slot)) & 3;
+        if (gone == 0 && pos + Cfg::UNIT <= clear) {
+          kv_attn_blocks<Cfg, Cfg::UNIT_BLOCKS, false>(st, blk, pos, cur.len, 0, lane);
+        } else {
 #pragma unroll 1
-        for (int i = 0; i < Cfg::UNIT_BLOCKS && pos + i * kKvBlockTokens < cur.len; ++i)
-          kv_attn_blocks<Cfg, 1, true>(st, blk + i * Blk::BYTES, pos + i * kKvBlockTokens, cur.len, (gone >> i) & 1, lane);
+          for (int i = 0; i < Cfg::UNIT_BLOCKS && pos + i * kKvBlockTokens < cur.len; ++i)
+            kv_attn_blocks<Cfg, 1, true>(st, blk + i * Blk::BYTES, pos + i * kKvBlockTokens, cur.len, (gone >> i) & 1, lane);
+        }
+        __syncwarp();  // every lane has read the slot
+        fetch(slot);
+        slot = slot + 1 == NSTAGE ? 0 : slot + 1;
       }
-      __syncwarp();  // every lane has read the slot
-      fetch(slot);
-      slot = slot + 1 == NSTAGE ? 0 : slot + 1;
+      // the accumulators go to the warp's partial result
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int row = nt * 8 + 2 * t + c;
+          const float down = kv_inverse(fabsf(st.wup[nt][c]));  // a factor of its own: with EVEN or ODD it may exceed fp32
+          if constexpr (Cfg::HALF) {
+#pragma unroll
+            for (int u = 0; u < D / 16; ++u) {
+              st.acc[u][nt][c] += __shfl_xor_sync(0xffffffffu, st.acc[u][nt][c], 2);
+              st.acc[u][nt][2 + c] += __shfl_xor_sync(0xffffffffu, st.acc[u][nt][2 + c], 2);
+            }
+          }
+          if (row < nrows) {
+            float* dst = part + (warp * part_rows + row) * PS + g * (D / 8);
+            const float f = first ? 0.f : kv_fall(st.m[nt][c] - stat[warp * ROWS + row]);  // what is there is for an older reference
+#pragma unroll
+            for (int u = 0; u < D / 16; u += 2) {
+              float4 x = make_float4(st.acc[u][nt][c] * EVEN * down, st.acc[u][nt][2 + c] * ODD * down,
+                                     st.acc[u + 1][nt][c] * EVEN * down, st.acc[u + 1][nt][2 + c] * ODD * down);
+              if (!first) {
+                const float4 y = *reinterpret_cast<const float4*>(dst + 2 * u);
+                x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+              }
+              *reinterpret_cast<float4*>(dst + 2 * u) = x;
+            }
+          }
+        }
+      __syncwarp();  // every lane has read the reference
+      if (g == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (nt * 8 + 2 * t + c < ROWS) stat[warp * ROWS + nt * 8 + 2 * t + c] = st.m[nt][c];
+      }
+      if (k >= kend) break;
     }
     const bool more = todo < mine;
     Part next;
@@ -737,35 +791,15 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     }
 
     // the four warps' partial results
-    const int g = lane >> 2, t = lane & 3;
-    const int nrows = min(ROWS, p.rows - cur.row0);
-    // what the numbers were taken for: odd channels of 4 bits times 16
-    constexpr float EVEN = Cfg::BITS == 4 && Cfg::SPLIT ? 16384.f : kKvLoUnit, ODD = Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float l = kv_sum_rows<Cfg::HALF>(st.l[nt][c]), z = kv_sum_rows<Cfg::HALF>(st.z[nt][c]);
         const int row = nt * 8 + 2 * t + c;
-        const float down = kv_inverse(fabsf(st.wup[nt][c]));  // a factor of its own: with EVEN or ODD it may exceed fp32
-        if constexpr (Cfg::HALF) {
-#pragma unroll
-          for (int u = 0; u < D / 16; ++u) {
-            st.acc[u][nt][c] += __shfl_xor_sync(0xffffffffu, st.acc[u][nt][c], 2);
-            st.acc[u][nt][2 + c] += __shfl_xor_sync(0xffffffffu, st.acc[u][nt][2 + c], 2);
-          }
-        }
         if (g == 0 && row < ROWS) {
-          stat[(0 * NW + warp) * ROWS + row] = st.m[nt][c];
           stat[(1 * NW + warp) * ROWS + row] = l;
           stat[(2 * NW + warp) * ROWS + row] = z;
-        }
-        if (row < nrows) {
-          float* dst = part + (warp * part_rows + row) * PS + g * (D / 8);
-#pragma unroll
-          for (int u = 0; u < D / 16; u += 2)
-            *reinterpret_cast<float4*>(dst + 2 * u) = make_float4(st.acc[u][nt][c] * EVEN * down, st.acc[u][nt][2 + c] * ODD * down,
-                                                                  st.acc[u + 1][nt][c] * EVEN * down, st.acc[u + 1][nt][2 + c] * ODD * down);
         }
       }
     __syncthreads();

@@ -15,8 +15,8 @@
 //   16-byte units of a lane are 512 bytes apart, so that a warp reads a unit of all lanes without bank conflicts and in one
 //     coalesced piece; the 8-byte quads of positions g and g + 8 are neighbours.
 // No byte holds numbers of two positions: a position is written without reading what is there.
-// V of odd positions is stored as N - n: the sums of the products then stay near zero, where the accumulators of the tensor cores,
-// which drop the bits that do not fit, lose the least (kv_attn.cuh).
+// V of odd positions is stored as N - n: the sums of the products of values about the middle of their ranges then stay near zero, where
+// the accumulators of the tensor cores, which drop the bits that do not fit, lose the least (kv_attn.cuh).
 #pragma once
 
 #include <cuda_bf16.h>

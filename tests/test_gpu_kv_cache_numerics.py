@@ -76,3 +76,27 @@ def test_values_near_the_largest_of_bf16(bits, group):
         want, want_lse, weight = attention64(q, held(k, bits), held(v, bits), i32(L), False, 1.0)
         assert o.isfinite().all()
         check_attn(o, lse, want, want_lse, weight)
+
+
+@pytest.mark.parametrize("group", [1, 4, 8, 16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_long_sequences_with_values_at_one_end_of_their_range(bits, group):
+    """One channel of V lies 40 above the others, so that these have the same few numbers everywhere and their sums grow all the way.
+    The accumulators of 1024 positions take 128 products (of 16 positions, in two pieces), each of which may drop less than 2^-23 of a sum
+    that grows to half of sum p range at most (numbers are added at even and subtracted at odd positions): 2^-18 of sum p range, here
+    2^-18 / 0.54 < 2^-17 of sum p 0.54 range, next to the tolerance of check_attn."""
+    L, B, d = 131072, 512, 64  # a head for every CTA: its four warps go over the whole sequence
+    g = torch.Generator("cuda").manual_seed(60)
+    k = 0.1 * torch.randn(1, 1, L, d, generator=g, device="cuda").half()
+    v = torch.randn(1, 1, L, d, generator=g, device="cuda")
+    v[..., 3] += 40
+    v = v.half()
+    cache, table = one_sequence(k, v, bits, 128, g)
+    q = torch.randn(B, group, 1, d, generator=g, device="cuda").half()
+    o = kv_cache_attn(q, cache, table.expand(B, -1), torch.full((B,), L, dtype=torch.int32, device="cuda"), None, False, d ** -0.5)
+    some = q[::171, :, 0].transpose(0, 1)[None]  # [1, group, 3, d]
+    want, _, weight = attention64(some, held(k, bits), held(v, bits), i32(L), False, d ** -0.5)
+    got = o[::171, :, 0].transpose(0, 1)[None].double()
+    size, spread = weight[..., :-1], weight[..., -1:]
+    tol = 2.0 ** -11 * want.abs() + 2.0 ** -14 * size + (2.0 ** -17 + 2.0 ** -22) * spread
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max().item()
