@@ -25,9 +25,10 @@
 // The accumulators of the tensor cores drop the bits that do not fit, always the same way. V of odd positions counts from the other end
 // (kv_format.cuh), so that both signs occur and the sums stay near zero where a channel's values lie about the middle of their rows'
 // ranges: 131072 positions in fp16 are then 2.1e-4 from 64 bits, all of it the rounding of the output, where numbers from 0 were 7e-3
-// off. For values at one end of the range, accumulators run over 1024 positions of a warp (HELD) and not over a sequence. With fp16 outputs a
-// probability goes through the tensor cores in two pieces (its fp16 value and what that leaves), with bf16 in one: one piece
-// alone is off by as much as rounding the output to fp16.
+// off. For values at one end of the range, accumulators run over 1024 positions of a warp (HELD) and not over a sequence. A
+// probability times its scale goes through the tensor cores in two pieces, its fp16 value and what that leaves: one piece alone is off by
+// as much as rounding the output to fp16, and turns one output in a few hundred to the other side of a rounding to bf16. Up to four rows
+// the second piece costs no product; beyond, it takes two bf16 rows of eight heads from 22.5 to 24.1 us, four from 32.9 to 37.5.
 //
 // Measured (B200, us, calls one after another; at the copy bandwidth): 8 sequences of 131072 positions, 32 heads over 8, d = 128, 4 bits,
 // fp16 200 (174), 5.7 TB/s; 2 of 16384, 16 heads, 8 bits, bf16 28.4 (21); 32 of up to 8192, 32 over 8, 4 bits, bf16 22.5 (10.8); 16 of
@@ -57,7 +58,6 @@ struct KvAttnConfig {
   static constexpr bool HALF = ROWS == 4;
   static constexpr int R = HALF ? 1 : 2;  // of positions g and g + 8, those a lane works on
   static constexpr bool BF16 = BF16_;
-  static constexpr bool SPLIT = !BF16;  // P in two pieces
   static constexpr int NWARPS = 4, NTHREADS = 32 * NWARPS;
   static constexpr int UNIT_BLOCKS = Blk::BYTES <= 2176 ? 2 : 1;  // a unit of work, and of the ring
   static constexpr int UNIT = UNIT_BLOCKS * kKvBlockTokens;       // positions
@@ -157,9 +157,7 @@ __device__ __forceinline__ uint32_t kv_nibble_lo(uint32_t x) { return x & 0x000f
 __device__ __forceinline__ uint32_t kv_nibble_hi(uint32_t x) { return x & 0x00f000f0u; }  // nibbles 1 and 5, times 16
 // The tensor cores line a subnormal up as if its leading bit were set, and drop what lies below the same place as for a number with
 // that bit. Of the even channels of V, n 2^-24 with n < 16, that is seen in an fp16 output: there it is n 2^-14.
-template <bool EXACT>
 __device__ __forceinline__ uint32_t kv_even(uint32_t x) {
-  if constexpr (!EXACT) return x;
   const uint32_t up = 0x64006400u;  // 2^10
   const __half2 r = __hmul2(reinterpret_cast<__half2&>(x), reinterpret_cast<const __half2&>(up));
   return reinterpret_cast<const uint32_t&>(r);
@@ -450,21 +448,20 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
           if (!EDGE || !hidden[nb][nt][i]) st.z[nt][c] = fmaf(x[nb][nt][i], vz[nb][r], st.z[nt][c]);
         }
         hi[r] = Kv16<false>::round2(w2[0], w2[1]);
-        if constexpr (Cfg::SPLIT) lo[r] = Kv16<false>::round2(w2[0] - Kv16<false>::lo(hi[r]), w2[1] - Kv16<false>::hi(hi[r]));
+        lo[r] = Kv16<false>::round2(w2[0] - Kv16<false>::lo(hi[r]), w2[1] - Kv16<false>::hi(hi[r]));
       }
       if constexpr (Cfg::HALF) {
         // Transposed, lanes of columns 0 to 3 have positions 0 to 7, those of columns 4 to 7 positions 8 to 15; the other places of
         // the fragment take the second pieces, which columns 4 to 7 and 0 to 3 then hold: all columns of a row are added at the end.
         const uint32_t most = kv_transpose8x8(hi[0]);
-        uint32_t rest = 0;
-        if constexpr (Cfg::SPLIT) rest = __shfl_xor_sync(0xffffffffu, kv_transpose8x8(lo[0]), 16);
+        const uint32_t rest = __shfl_xor_sync(0xffffffffu, kv_transpose8x8(lo[0]), 16);
         pb[nb][nt][0] = lane < 16 ? most : rest;
         pb[nb][nt][1] = lane < 16 ? rest : most;
       } else {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           pb[nb][nt][r] = kv_transpose8x8(hi[r]);
-          if constexpr (Cfg::SPLIT) pl[nb][nt][r] = kv_transpose8x8(lo[r]);
+          pl[nb][nt][r] = kv_transpose8x8(lo[r]);
         }
       }
     }
@@ -488,9 +485,9 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         uint32_t f[4];
         if constexpr (BITS == 4) {
           const uint32_t p0 = i & 1 ? ab[i >> 1] >> 8 : ab[i >> 1], p1 = i & 1 ? cd[i >> 1] >> 8 : cd[i >> 1];
-          f[0] = kv_even<Cfg::SPLIT>(kv_nibble_lo(p0));
+          f[0] = kv_even(kv_nibble_lo(p0));
           f[1] = kv_nibble_hi(p0);
-          f[2] = kv_even<Cfg::SPLIT>(kv_nibble_lo(p1));
+          f[2] = kv_even(kv_nibble_lo(p1));
           f[3] = kv_nibble_hi(p1);
         } else {
           f[0] = kv_bytes(ab[i], 0x4240);
@@ -502,7 +499,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         for (int nt = 0; nt < NT; ++nt) {
           float* acc = st.acc[TILES * v + i][nt];
           kv_mma(acc, f, pb[nb][nt], acc);
-          if constexpr (Cfg::SPLIT && !Cfg::HALF) kv_mma(acc, f, pl[nb][nt], acc);
+          if constexpr (!Cfg::HALF) kv_mma(acc, f, pl[nb][nt], acc);
         }
       }
     }
@@ -720,7 +717,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int g = lane >> 2, t = lane & 3;
     const int nrows = min(ROWS, p.rows - cur.row0);
     // what the numbers were taken for: odd channels of 4 bits times 16
-    constexpr float EVEN = Cfg::BITS == 4 && Cfg::SPLIT ? 16384.f : kKvLoUnit, ODD = Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit;
+    constexpr float EVEN = Cfg::BITS == 4 ? 16384.f : kKvLoUnit, ODD = Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit;
     for (bool first = true;; first = false) {
 #pragma unroll
       for (int u = 0; u < D / 16; ++u)

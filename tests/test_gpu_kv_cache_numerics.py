@@ -100,3 +100,26 @@ def test_long_sequences_with_values_at_one_end_of_their_range(bits, group):
     size, spread = weight[..., :-1], weight[..., -1:]
     tol = 2.0 ** -11 * want.abs() + 2.0 ** -14 * size + (2.0 ** -17 + 2.0 ** -22) * spread
     assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("group", [2, 8, 16])
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_values_that_cancel(bits, name, group):
+    """Two positions with opposite values and nearly the same probability: the output is a small difference, whose own rounding hides
+    nothing of how the probabilities went through the products (in two pieces: 2^-22 of the values; in one: up to 2^-12)."""
+    dtype, d, B = DT[name], 128, 40
+    g = torch.Generator("cuda").manual_seed(70)
+    k = torch.randn(B, 1, 2, d, generator=g, device="cuda").to(dtype)
+    v = torch.randn(B, 1, 1, d, generator=g, device="cuda").to(dtype)
+    v = torch.cat([v, -v], 2)
+    table, pages = tables(g, B, 1)
+    cache = QuantizedKVCache(pages, 1, d, bits=bits, page_size=16, dtype=dtype)
+    kv_cache_write(cache, k, v, table, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    q = (0.002 * torch.randn(B, group, 1, d, generator=g, device="cuda")).to(dtype)
+    lengths = torch.full((B,), 2, dtype=torch.int32, device="cuda")
+    o, lse = kv_cache_attn(q, cache, table, lengths, None, False, 1.0, True)
+    want, _, weight = attention64(q, held(k, bits), held(v, bits), lengths, False, 1.0)
+    size, spread = weight[..., :-1], weight[..., -1:]
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -14 * size + 2.0 ** -22 * spread
+    assert ((o.double() - want).abs() <= tol).all(), ((o.double() - want).abs() / tol).max().item()
