@@ -123,3 +123,35 @@ def test_values_that_cancel(bits, name, group):
     size, spread = weight[..., :-1], weight[..., -1:]
     tol = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -14 * size + 2.0 ** -22 * spread
     assert ((o.double() - want).abs() <= tol).all(), ((o.double() - want).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("group", [1, 8, 16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scores_with_outlying_channels(bits, name, d, group):
+    """Sequences of one position, so that lse is the score: one channel of q is 40 to 80 and one of K 200, or of positive K 30, where the
+    others are 1, which leaves few numbers for the others. A score is scale (ks sum q n + kz sum q), its products d / 16 sums of 16, each of which may
+    drop less than 2^-23 of the largest partial sum, and eight roundings of 2^-24 for the rest, all relative to scale times
+    M = sum |q| (n ks + |kz|); exp2 and log2 units add 2^-22 of the score."""
+    dtype, B = DT[name], 64
+    g = torch.Generator("cuda").manual_seed(80)
+    for at, far in ((4, 200.0), (5, 200.0), (10, 30.0), (11, 30.0), (d - 1, 200.0)):  # nibbles of either kind
+        q = torch.randn(B, group, 1, d, generator=g, device="cuda")
+        q[..., at] = 40 * (1 + torch.rand(B, group, 1, generator=g, device="cuda"))
+        k = torch.randn(B, 1, 1, d, generator=g, device="cuda")
+        if far < 100:
+            k = k.abs()
+        k[..., (at + 13) % d] = far
+        q, k = q.to(dtype), k.to(dtype)
+        table, pages = tables(g, B, 1)
+        cache = QuantizedKVCache(pages, 1, d, bits=bits, page_size=16, dtype=dtype)
+        kv_cache_write(cache, k, k, table, torch.zeros(B, dtype=torch.int32, device="cuda"))
+        one = torch.ones(B, dtype=torch.int32, device="cuda")
+        _, lse = kv_cache_attn(q, cache, table, one, None, False, d ** -0.5, True)
+        hk = held(k, bits)
+        want = (q.double() * hk).sum(-1) * d ** -0.5
+        low = hk.amin(-1, keepdim=True)
+        size = (q.double().abs() * (hk - low + low.abs())).sum(-1) * d ** -0.5
+        tol = (d / 16 + 8) * 2.0 ** -23 * size + 2.0 ** -22 * want.abs()
+        assert ((lse.double() - want).abs() <= tol).all(), ((lse.double() - want).abs() / tol).max().item()
