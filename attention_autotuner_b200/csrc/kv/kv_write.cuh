@@ -222,25 +222,21 @@ struct KvReadParams {
 template <int BITS, bool BF16>
 __device__ __forceinline__ uint4 kv_values8(const uint32_t* w, uint32_t meta) {
   using T = Kv16<BF16>;
-  if constexpr (BITS == 8 && BF16) {  // 128 + n takes eight bits behind the leading one, and a bf16 has seven
-    const float s = T::lo(meta), z = T::hi(meta);
-    uint32_t r[4];
+  // n in the mantissa of 1024 (bf16: 128; with 8 bits 2^23 in fp32, since a bf16 has seven bits behind the leading one), an exact
+  // difference, and one packed fma
+  constexpr uint32_t BASE = BF16 ? 0x43004300u : 0x64006400u;
+  const uint32_t s2 = __byte_perm(meta, meta, 0x1010), z2 = __byte_perm(meta, meta, 0x3232);
+  uint32_t n[4];
+  if constexpr (BITS == 8 && BF16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float f[2];
+      uint32_t f[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float n = __uint_as_float(__byte_perm(w[i >> 1], 0x4b000000u, 0x7440 + 2 * (i & 1) + j)) - 8388608.f;  // 2^23 + n
-        f[j] = fmaf(n, s, z);  // the product is exact, 8 by 8 bits
-      }
-      r[i] = T::round2(f[0], f[1]);
+      for (int j = 0; j < 2; ++j)
+        f[j] = __float_as_uint(__uint_as_float(__byte_perm(w[i >> 1], 0x4b000000u, 0x7440 + 2 * (i & 1) + j)) - 8388608.f);
+      n[i] = __byte_perm(f[0], f[1], 0x7632);  // the upper halves: n has eight bits
     }
-    return make_uint4(r[0], r[1], r[2], r[3]);
   } else {
-    // n in the mantissa of 1024 (bf16: 128), an exact difference, and one packed fma
-    constexpr uint32_t BASE = BF16 ? 0x43004300u : 0x64006400u;
-    const uint32_t s2 = __byte_perm(meta, meta, 0x1010), z2 = __byte_perm(meta, meta, 0x3232);
-    uint32_t n[4];
     if constexpr (BITS == 4) {
       // nibbles 0 and 4, 1 and 5, ...; put back in order below
 #pragma unroll
@@ -250,11 +246,13 @@ __device__ __forceinline__ uint4 kv_values8(const uint32_t* w, uint32_t meta) {
       for (int i = 0; i < 4; ++i) n[i] = __byte_perm(w[i >> 1], BASE, i & 1 ? 0x7372 : 0x7170);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = T::fma2(T::sub2(n[i], BASE), s2, z2);
-    if constexpr (BITS == 8) return make_uint4(n[0], n[1], n[2], n[3]);
-    return make_uint4(__byte_perm(n[0], n[1], 0x5410), __byte_perm(n[2], n[3], 0x5410), __byte_perm(n[0], n[1], 0x7632),
-                      __byte_perm(n[2], n[3], 0x7632));
+    for (int i = 0; i < 4; ++i) n[i] = T::sub2(n[i], BASE);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) n[i] = T::fma2(n[i], s2, z2);
+  if constexpr (BITS == 8) return make_uint4(n[0], n[1], n[2], n[3]);
+  return make_uint4(__byte_perm(n[0], n[1], 0x5410), __byte_perm(n[2], n[3], 0x5410), __byte_perm(n[0], n[1], 0x7632),
+                    __byte_perm(n[2], n[3], 0x7632));
 }
 template <int BITS>
 __device__ __forceinline__ void kv_load_words(const uint8_t* from, uint32_t* w) {

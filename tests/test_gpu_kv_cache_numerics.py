@@ -4,9 +4,9 @@ import math
 
 import pytest
 import torch
-from test_gpu_kv_cache import DT, attention64, check_attn, held, i32, tables
+from test_gpu_kv_cache import DT, FORMS, attention64, check_attn, held, i32, tables
 
-from attention_autotuner_b200.ops.cache_interface import QuantizedKVCache, kv_cache_attn, kv_cache_write
+from attention_autotuner_b200.ops.cache_interface import QuantizedKVCache, kv_cache_attn, kv_cache_read, kv_cache_write
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,24 @@ def test_scores_with_outlying_channels(bits, name, d, group):
         size = (q.double().abs() * (hk - low + low.abs())).sum(-1) * d ** -0.5
         tol = (d / 16 + 8) * 2.0 ** -23 * size + 2.0 ** -22 * want.abs()
         assert ((lse.double() - want).abs() <= tol).all(), ((lse.double() - want).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("bits,d,name", FORMS)
+def test_values_read_back_are_rounded_once(bits, d, name):
+    """Rows of positive values whose smallest is far below the step: about one product of a scale and a number in 2^8 lies half way between
+    two 16-bit values, and the zero decides. Against zero + scale n in 64 bits (exact: 40 bits), rounded half to even by its bits;
+    .to(dtype) would round to 32 bits on the way."""
+    dtype, L = DT[name], 1000
+    g = torch.Generator("cuda").manual_seed(90)
+    x = torch.rand(1, 2, L, d, generator=g, device="cuda") * torch.exp2(torch.randint(0, 5, (1, 2, L, 1), generator=g, device="cuda").float()) + 0.5
+    x[..., 7] = 2.0 ** (-14 if name == "fp16" else -24) * (1 + torch.rand(1, 2, L, generator=g, device="cuda"))
+    x = x.to(dtype)
+    cache, table = one_sequence(x, x.flip(1), bits, 64, g)
+    k, v = kv_cache_read(cache, table, None, None, L)
+    low, high = x.float().amin(-1, keepdim=True), x.float().amax(-1, keepdim=True)
+    step = ((high - low) / torch.full_like(low, 2 ** bits - 1)).to(dtype).float()
+    n = ((x.float() - low) / step).round().clamp(max=2 ** bits - 1)  # in fp32, as the format has it
+    m, e = torch.frexp(low.double() + step.double() * n.double())
+    digits = 2 / torch.finfo(dtype).eps
+    want = torch.ldexp(torch.round(m * digits) / digits, e)
+    assert torch.equal(k.double(), want) and torch.equal(v.double(), want.flip(1))
