@@ -129,7 +129,7 @@ __device__ __forceinline__ int kv_length(const KvAttnParams& p, int b, bool repo
   const int n = p.lengths[b];
   const long long room = static_cast<long long>(p.cache.table_width) << p.cache.page_shift;
   if (n >= 0 && n <= room) return n;
-  if (report) kv_report(kKvBadLength, b);
+  if (report) kv_report(kKvBadLength, p.cache.first + b);
   return n < 0 ? 0 : static_cast<int>(room);
 }
 template <int UNIT>

@@ -162,28 +162,46 @@ size_t kv_attn_ws_bytes(int rows, long long positions) {
 template <class Cfg>
 int kv_attn_launch(KvAttnParams p, size_t ws_bytes, cudaStream_t stream) {
   p.row_blocks = (p.rows + Cfg::ROWS - 1) / Cfg::ROWS;
-  const long long items = static_cast<long long>(p.B) * p.cache.heads * p.row_blocks;
+  // The kernels count work in 32 bits (and kv_div), for tables as full as they can be: the lengths are on the device. A batch that
+  // could hold more goes out in several launches, one after another with the same workspace.
+  const long long per_seq = static_cast<long long>(p.cache.heads) * p.row_blocks;
   const long long units = (static_cast<long long>(p.cache.table_width) << p.cache.page_shift) / Cfg::UNIT + 1 + kKvHeadCost<Cfg::UNIT>;
-  if (items > 0x7fffffff / units || static_cast<long long>(p.cache.heads) * p.row_blocks > 1 << 20)  // 32-bit numbers, kv_div
-    return fail(kErrInvalidArgument, "kv_attn: %d sequences x %d heads x %d row blocks with tables of %d pages exceed 2^31 units of work", p.B,
-                p.cache.heads, p.row_blocks, p.cache.table_width);
+  const long long most = 0x7fffffff / (per_seq * units);
+  if (most == 0 || per_seq > 1 << 20)
+    return fail(kErrInvalidArgument, "kv_attn: %d heads x %d row blocks with tables of %d pages exceed 2^31 units of work", p.cache.heads,
+                p.row_blocks, p.cache.table_width);
   const int grid = kv_attn_grid<Cfg>(p.rows);
   const size_t need = kv_attn_ws_bytes<Cfg>(p.rows, static_cast<long long>(p.cache.table_width) << p.cache.page_shift);
   if (ws_bytes < need || (need > 0 && p.ws == nullptr))
     return fail(kErrInvalidArgument, "kv_attn: %zu bytes of workspace, %zu are needed", p.ws == nullptr ? size_t(0) : ws_bytes, need);
-  const int smem = Cfg::smem_bytes(p.rows, p.B);
   p.by_grid = make_fast_div(grid);
   p.whole = kv_attn_whole(static_cast<long long>(p.cache.table_width) << p.cache.page_shift, Cfg::D);
   auto kernel = &kv_attn_kernel<Cfg>;
   cudaError_t e = kv_attn_allow_smem<Cfg>();
   if (e != cudaSuccess) return fail(kErrCuda, "kv_attn: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  if (int rc = kv_launch("kv_attn", kernel, dim3(grid, 1, 1), Cfg::NTHREADS, smem, stream, p)) return rc;
-  if (p.whole) return kOk;
-  // tasks of a head: a block of its own for each where there are few heads (one may lie in all runs), a warp where there are many
-  const int tasks = std::min(p.rows, Cfg::ROWS) * (Cfg::D / 64);
-  const bool few = items * tasks <= 2 * kv_sms();
-  return kv_launch("kv_attn", &kv_attn_join_kernel<Cfg::D, Cfg::ROWS, Cfg::UNIT, Cfg::BF16>,
-                   dim3(static_cast<unsigned>(items), static_cast<unsigned>(few ? tasks : (tasks + 7) / 8), 1), few ? 512 : 256, 0, stream, p, grid);
+  const int B = p.B, launches = static_cast<int>((B + most - 1) / most), each = (B + launches - 1) / launches;
+  const long long rows = static_cast<long long>(p.cache.heads) * p.rows;  // of a sequence
+  for (int b = 0; b < B; b += each) {
+    KvAttnParams x = p;
+    x.B = std::min(each, B - b);
+    x.cache.first = b;
+    x.cache.table += static_cast<long long>(b) * p.cache.table_stride;
+    x.lengths += b;
+    x.q = static_cast<const uint16_t*>(p.q) + b * rows * Cfg::D;
+    x.o = static_cast<uint16_t*>(p.o) + b * rows * Cfg::D;
+    if (p.lse != nullptr) x.lse += b * rows;
+    if (int rc = kv_launch("kv_attn", kernel, dim3(grid, 1, 1), Cfg::NTHREADS, Cfg::smem_bytes(p.rows, x.B), stream, x)) return rc;
+    if (p.whole) continue;
+    // tasks of a head: a block of its own for each where there are few heads (one may lie in all runs), a warp where there are many
+    const long long items = x.B * per_seq;
+    const int tasks = std::min(p.rows, Cfg::ROWS) * (Cfg::D / 64);
+    const bool few = items * tasks <= 2 * kv_sms();
+    if (int rc = kv_launch("kv_attn", &kv_attn_join_kernel<Cfg::D, Cfg::ROWS, Cfg::UNIT, Cfg::BF16>,
+                           dim3(static_cast<unsigned>(items), static_cast<unsigned>(few ? tasks : (tasks + 7) / 8), 1), few ? 512 : 256, 0,
+                           stream, x, grid))
+      return rc;
+  }
+  return kOk;
 }
 
 template <class F>

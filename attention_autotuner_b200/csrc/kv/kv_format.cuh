@@ -62,16 +62,17 @@ struct KvCacheView {
   long long head_bytes;      // one head of one page
   int table_stride, table_width;
   int num_pages, heads, page_shift;  // page_size = 1 << page_shift
+  int first;                         // the call's number of the first sequence that this launch works on
 };
 
 // What a kernel found in the tables that it was given (the host cannot see them). The kernels leave such positions out: not
 // written, read back as zeros, not attended to. Sticky like the status words of ptx.cuh, with the fourth word of the same mirror.
 enum KvBad : int { kKvBadPage = 1, kKvBadLength = 2 };
 __device__ int g_kv_bad = 0;
-__device__ __noinline__ void kv_report(int what, int b) {
+__device__ __noinline__ void kv_report(int what, int sequence) {
   if (atomicCAS(&g_kv_bad, 0, what) == 0) {
     volatile int* mirror = g_status_mirror;
-    if (mirror != nullptr) mirror[3] = what | (b << 8);
+    if (mirror != nullptr) mirror[3] = what | (sequence << 8);
   }
 }
 
@@ -79,12 +80,12 @@ __device__ __noinline__ void kv_report(int what, int b) {
 __device__ __forceinline__ int kv_page(const KvCacheView& c, int b, int pos) {
   const int i = pos >> c.page_shift;
   if (i >= c.table_width) {
-    kv_report(kKvBadLength, b);
+    kv_report(kKvBadLength, c.first + b);
     return -1;
   }
   const int page = c.table[static_cast<long long>(b) * c.table_stride + i];
   if (page < 0 || page >= c.num_pages) {
-    kv_report(kKvBadPage, b);
+    kv_report(kKvBadPage, c.first + b);
     return -1;
   }
   return page;

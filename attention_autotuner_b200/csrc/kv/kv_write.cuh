@@ -26,7 +26,7 @@ __device__ __forceinline__ int kv_count(const KvCacheView& c, int count, int sta
   if (count == 0) return 0;
   const int room = static_cast<int>(static_cast<long long>(c.table_width) << c.page_shift);  // below 2^31 - 31, the host checks
   if (count > 0 && count <= L && start >= 0 && start <= room - count) return count;
-  if (threadIdx.x == 0) kv_report(kKvBadLength, b);
+  if (threadIdx.x == 0) kv_report(kKvBadLength, c.first + b);
   return start < 0 || start >= room ? 0 : min(min(max(count, 0), L), room - start);
 }
 

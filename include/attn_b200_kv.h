@@ -61,8 +61,9 @@ int attn_b200_kv_read(const attn_b200_kv_cache* cache, const int* table, int tab
  * [B, heads * group, Lq, head_dim] dense, query heads h * group ... of head h; lse [B, heads * group, Lq] or NULL. causal: query i
  * sees position j <= i + lengths[b] - Lq. A query that sees none gets 0 and -inf. Lq up to ATTN_B200_KV_MAX_QUERIES, B up to 4096.
  * workspace: attn_b200_kv_attn_workspace_bytes() bytes (0 where tables hold few positions; then NULL will do), 16-byte aligned,
- * contents undefined before and after; two calls that may run at the same time need one each. One or two launches. The same call
- * gives the same bits. */
+ * contents undefined before and after; two calls that may run at the same time need one each. One or two launches, or that for each
+ * part of a batch whose tables could hold more than 2^31 units of work (32 or 16 positions of a head for up to 16 rows); a single
+ * sequence whose table could hold more is refused. The same call gives the same bits. */
 size_t attn_b200_kv_attn_workspace_bytes(const attn_b200_kv_cache* cache, int table_width, int B, int group, int Lq);
 int attn_b200_kv_attn(const void* q, const attn_b200_kv_cache* cache, const int* table, int table_stride, int table_width,
                       const int* lengths, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int group, int Lq,

@@ -6,6 +6,7 @@ import pytest
 import torch
 from test_gpu_kv_cache import DT, FORMS, attention64, check_attn, held, i32, tables
 
+from attention_autotuner_b200 import _lib
 from attention_autotuner_b200.ops.cache_interface import QuantizedKVCache, kv_cache_attn, kv_cache_read, kv_cache_write
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +177,31 @@ def test_values_read_back_are_rounded_once(bits, d, name):
     digits = 2 / torch.finfo(dtype).eps
     want = torch.ldexp(torch.round(m * digits) / digits, e)
     assert torch.equal(k.double(), want) and torch.equal(v.double(), want.flip(1))
+
+
+def test_tables_that_could_hold_more_than_the_kernels_count():
+    """Rows of 32767 pages of 65536 positions for 40 sequences of ordinary lengths: several launches, each of which counts in 32 bits, and
+    a page that does not exist is reported with its own sequence."""
+    B, H, d, page, width = 40, 2, 64, 65536, 32767
+    g = torch.Generator("cuda").manual_seed(100)
+    L = 70000
+    k, v = (torch.randn(2, H, L, d, generator=g, device="cuda").half() for _ in range(2))
+    cache = QuantizedKVCache(4, H, d, bits=4, page_size=page)
+    two = i32(2, 0, 1, 3).reshape(2, 2)
+    kv_cache_write(cache, k, v, two, i32(0, 0))
+    table = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = two.repeat(B // 2, 1)
+    lengths = torch.tensor([(0, 1, 33, 511, 5000, 65536, 65537, L)[i % 8] for i in range(B)], dtype=torch.int32, device="cuda")
+    q = torch.randn(B, 3 * H, 1, d, generator=g, device="cuda").half()
+    o, lse = kv_cache_attn(q, cache, table, lengths, None, True, 0.125, True)
+    hk, hv = held(k, 4), held(v, 4)
+    for b in range(B):
+        at = slice(b, b + 1), slice(b % 2, b % 2 + 1)
+        check_attn(o[at[0]], lse[at[0]], *attention64(q[at[0]], hk[at[1]], hv[at[1]], lengths[at[0]], True, 0.125))
+    assert _lib.kv_status() == 0
+    table[33, 0] = 4
+    kv_cache_attn(q, cache, table, lengths)
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.AttnB200Error, match="sequence 33"):
+        kv_cache_attn(q, cache, table, lengths)
+    assert _lib.kv_status() == 3
