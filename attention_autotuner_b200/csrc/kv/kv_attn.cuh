@@ -312,19 +312,20 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
   constexpr int R = Cfg::R;
   const int own = Cfg::HALF ? (lane & 2) * 4 : 0;  // the first position of this lane is g + own
 
-  float s[NB][NT][2 * R];
-  float ks[NB][R], kz[NB][R], vs[NB][R], vz[NB][R];  // of the lane's positions; vz: what V stands for with its numbers 0
+  float y[NB][NT][2 * R];              // scores, in exp2 units
+  float vs[NB][R], vz[NB][R];  // of the lane's positions; vz: what V stands for with its numbers 0
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const uint8_t* at = blk + nb * Blk::BYTES;
+    float ks[R], kz[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       uint2 meta = *reinterpret_cast<const uint2*>(at + Blk::META + g * 16 + own + 8 * r);
       if constexpr (EDGE) {  // what lies behind the length is whatever was in the page
         if (((missing >> nb) & 1) || pos0 + nb * 16 + g + own + 8 * r >= len) meta = make_uint2(0, 0);
       }
-      ks[nb][r] = T::lo(meta.x);
-      kz[nb][r] = T::hi(meta.x);
+      ks[r] = T::lo(meta.x);
+      kz[r] = T::hi(meta.x);
       vs[nb][r] = T::lo(meta.y);
       vz[nb][r] = fmaf(st.vflip, vs[nb][r], T::hi(meta.y));
     }
@@ -360,7 +361,8 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 2 * R; ++i) s[nb][nt][i] = Cfg::HALF && own ? sum[nt][i + 2] : sum[nt][i];
+      for (int i = 0; i < 2 * R; ++i)
+        y[nb][nt][i] = fmaf(ks[i >> 1] * st.cq[nt][i & 1], Cfg::HALF && own ? sum[nt][i + 2] : sum[nt][i], kz[i >> 1] * st.sq[nt][i & 1]);
   }
 
   // probabilities against the present references, and weights of the numbers of V
@@ -374,7 +376,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i) {
           const int r = i >> 1, c = i & 1;  // position g + own + 8 r, the lane's column c
-          e[nb][nt][i] = fmaf(ks[nb][r] * st.cq[nt][c], s[nb][nt][i], fmaf(kz[nb][r], st.sq[nt][c], -st.m[nt][c]));
+          e[nb][nt][i] = y[nb][nt][i] - st.m[nt][c];  // of the very number that the reference comes from: below 0 whatever its size
           if constexpr (EDGE) {
             hidden[nb][nt][i] = ((missing >> nb) & 1) || pos0 + nb * 16 + g + own + 8 * r >= st.lim[nt][c];
             if (hidden[nb][nt][i]) e[nb][nt][i] = -INFINITY;
@@ -407,9 +409,8 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
           for (int r = 0; r < R; ++r) {
             const int i = 2 * r + c;
             if (EDGE && hidden[nb][nt][i]) continue;
-            const float y = fmaf(ks[nb][r] * st.cq[nt][c], s[nb][nt][i], kz[nb][r] * st.sq[nt][c]);
-            top = fmaxf(top, y);
-            wide = fmaxf(wide, y + __log2f(vs[nb][r]));
+            top = fmaxf(top, y[nb][nt][i]);
+            wide = fmaxf(wide, y[nb][nt][i] + __log2f(vs[nb][r]));
           }
         // The reference is a whole number, so that what it moves by is taken out of the sums exactly.
         const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)) + kKvBelow);

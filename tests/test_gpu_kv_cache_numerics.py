@@ -205,3 +205,30 @@ def test_tables_that_could_hold_more_than_the_kernels_count():
     with pytest.raises(_lib.AttnB200Error, match="sequence 33"):
         kv_cache_attn(q, cache, table, lengths)
     assert _lib.kv_status() == 3
+
+
+@pytest.mark.parametrize("group", [1, 8, 16])
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scores_of_any_size(bits, name, group):
+    """Scores up to 1e10, where a step of fp32 is 1000: the largest takes all, and the output is its value, rounded."""
+    dtype, d, B = DT[name], 128, 100
+    g = torch.Generator("cuda").manual_seed(110)
+    sign = torch.where(torch.rand(B, 1, 1, d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    q = 6e4 * sign * (0.5 + 0.5 * torch.rand(B, group, 1, d, generator=g, device="cuda"))
+    k = 6e4 * sign * torch.tensor([0.2, 1.0, 0.5, -1.0], device="cuda")[:, None] * (0.9 + 0.1 * torch.rand(B, 1, 4, d, generator=g, device="cuda"))
+    v = torch.randn(B, 1, 4, d, generator=g, device="cuda")
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    table, pages = tables(g, B, 1)
+    cache = QuantizedKVCache(pages, 1, d, bits=bits, page_size=16, dtype=dtype)
+    kv_cache_write(cache, k, v, table, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    lengths = torch.full((B,), 4, dtype=torch.int32, device="cuda")
+    o, lse = kv_cache_attn(q, cache, table, lengths, None, False, d ** -0.5, True)
+    want, want_lse, _ = attention64(q, held(k, bits), held(v, bits), lengths, False, d ** -0.5)
+    assert want_lse.min() > 1e9
+    hv = held(v, bits)[:, :, 1:2].expand_as(want)
+    assert torch.equal(want, hv)
+    # the value is put together of scale n and zero, each with a rounding of fp32 (the scale in pieces of 2^-22)
+    rng = held(v, bits).amax(-1, keepdim=True)[:, :, 1:2] - held(v, bits).amin(-1, keepdim=True)[:, :, 1:2]
+    assert ((o.double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -21 * rng).all()
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -18 * want_lse).all()  # 16 products of 2^-23, a few roundings of 2^-24, of scores that do not cancel
