@@ -58,6 +58,9 @@ struct KvAttnConfig {
   static constexpr bool HALF = ROWS == 4;
   static constexpr int R = HALF ? 1 : 2;  // of positions g and g + 8, those a lane works on
   static constexpr bool BF16 = BF16_;
+  // The sums of V are kept times this until they are divided: below the largest fp32 number for every finite bf16 value, up to half a
+  // million positions. bf16 values lose bits below 2^-117 for it.
+  static constexpr float VDOWN = BF16 ? 1.f / 16777216.f : 1.f, VUP = 1.f / VDOWN;
   static constexpr int NWARPS = 4, NTHREADS = 32 * NWARPS;
   static constexpr int UNIT_BLOCKS = Blk::BYTES <= 2176 ? 2 : 1;  // a unit of work, and of the ring
   static constexpr int UNIT = UNIT_BLOCKS * kKvBlockTokens;       // positions
@@ -73,7 +76,10 @@ struct KvAttnConfig {
   static constexpr int STAT_BYTES = 3 * NWARPS * ROWS * 4;  // reference, sum, sum of p vz
   static constexpr int Q_BYTES = 8 * NT * (D * 2 + 16);  // fragments, and what kv_store_q says of a row
   static constexpr int Q_PASSES = (ROWS * D / 8 + NTHREADS - 1) / NTHREADS;
-  static constexpr int MIN_CTAS = NT * D <= 128 ? 3 : 2;  // 168 or 255 registers
+  // 168 or 255 registers. d = 64 with 16 rows spills up to 104 bytes at 168; with two CTAs per SM and no spills a draft of four (16 of up to
+  // 4096, 8 bits) takes 12.7 us instead of 12.9, four of a ragged batch (4 bits, bf16) 26.0 instead of 26.4, four of 131072 positions in 8 bits
+  // 134.7 instead of 129.4.
+  static constexpr int MIN_CTAS = NT * D <= 128 ? 3 : 2;
   static constexpr int part_bytes(int rows) { return NWARPS * (rows < ROWS ? rows : ROWS) * PART_STRIDE * 4; }
   static int smem_bytes(int rows, int B) { return RING_BYTES + Q_BYTES + STAT_BYTES + part_bytes(rows) + (B + 1) * 8; }
 };
@@ -186,10 +192,6 @@ __device__ __forceinline__ float kv_weight(float m, float l, float M) {
   return ex2_approx(m - M);
 }
 
-// The reference lies this much above the largest score (in exp2 units): the sums of a row, not yet divided, then stay below 2^-20 times
-// positions times the largest value, in fp32 for every finite bf16 value up to a million positions. What lies 2^102 below the largest
-// probability is lost for it, and scales of V lose bits below 2^-94.
-constexpr float kKvBelow = 24.f;
 // 2^-x of a whole number x from 0; 0 beyond 126, and of NaN (from -inf to -inf).
 __device__ __forceinline__ float kv_fall(float x) {
   return __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(fminf(x, 127.f))) << 23);
@@ -327,7 +329,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
       ks[r] = T::lo(meta.x);
       kz[r] = T::hi(meta.x);
       vs[nb][r] = T::lo(meta.y);
-      vz[nb][r] = fmaf(st.vflip, vs[nb][r], T::hi(meta.y));
+      vz[nb][r] = fmaf(st.vflip, vs[nb][r], T::hi(meta.y)) * Cfg::VDOWN;
     }
     uint32_t w[LANE_UNITS * 4];
 #pragma unroll
@@ -396,7 +398,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
         etop = fmax3(etop, e[nb][nt][2 * r], e[nb][nt][2 * r + 1]);
         wtop = fmax3(wtop, fabsf(wt[nb][nt][2 * r]), fabsf(wt[nb][nt][2 * r + 1]));
       }
-  if (__any_sync(0xffffffffu, etop > 4.f - kKvBelow || wtop > 16384.f)) {
+  if (__any_sync(0xffffffffu, etop > 4.f || wtop > 16384.f)) {
     // per column: the largest score, and the largest score plus logarithm of a scale of V, from the scores themselves
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -413,7 +415,7 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
             wide = fmaxf(wide, y[nb][nt][i] + __log2f(vs[nb][r]));
           }
         // The reference is a whole number, so that what it moves by is taken out of the sums exactly.
-        const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)) + kKvBelow);
+        const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)));
         wide = kv_max_rows<Cfg::HALF>(wide) - mn;  // of the largest weight
         const int drop = static_cast<int>(fminf(mn - st.m[nt][c], 252.f));  // 252 from -inf too, and where nothing was seen yet
         const float f = kv_fall(mn - st.m[nt][c]);
@@ -721,7 +723,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
     const int g = lane >> 2, t = lane & 3;
     const int nrows = min(ROWS, p.rows - cur.row0);
     // what the numbers were taken for: odd channels of 4 bits times 16
-    constexpr float EVEN = Cfg::BITS == 4 ? kKvUnit : kKvLoUnit, ODD = Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit;
+    constexpr float EVEN = (Cfg::BITS == 4 ? kKvUnit : kKvLoUnit) * Cfg::VDOWN, ODD = (Cfg::BITS == 4 ? kKvHiUnit : kKvLoUnit) * Cfg::VDOWN;
     for (bool first = true;; first = false) {
 #pragma unroll
       for (int u = 0; u < D / 16; ++u)
@@ -830,7 +832,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
       x.z += Z;
       x.w += Z;
       if (whole) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float inv = L == 0.f ? 0.f : 1.f / L * Cfg::VUP;
         const long long row_at = cur.q_row0 + cur.row0 + row;
         reinterpret_cast<uint2*>(p.o)[row_at * (D / 4) + c4] = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
         if (p.lse != nullptr && c4 == 0) p.lse[row_at] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
@@ -857,6 +859,7 @@ __global__ void __launch_bounds__(Cfg::NTHREADS, Cfg::MIN_CTAS) kv_attn_kernel(c
 template <int D, int ROWS, int UNIT, bool BF16>
 __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant__ KvAttnParams p, int grid) {
   using T = Kv16<BF16>;
+  constexpr float VUP = KvAttnConfig<4, D, ROWS, BF16>::VUP;
   constexpr int STRIDE = ROWS * (D + 2);
   __shared__ float2 weight[kKvMaxRuns];  // of a part: reference, then weight; sum
   __shared__ float red[2][16];
@@ -910,7 +913,7 @@ __global__ void __launch_bounds__(512) kv_attn_join_kernel(const __grid_constant
   const int tasks = nrows * PAIRS;
   const long long out0 = (static_cast<long long>(b) * p.cache.heads + item / p.row_blocks) * p.rows + row0;
   auto store = [&](int row, int pair, float2 x, float L) {
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const float inv = L == 0.f ? 0.f : 1.f / L * VUP;
     reinterpret_cast<uint32_t*>(p.o)[(out0 + row) * (D / 2) + pair * 32 + lane] = T::round2(x.x * inv, x.y * inv);
   };
   auto store_lse = [&](int row, float M, float L) {

@@ -232,3 +232,19 @@ def test_scores_of_any_size(bits, name, group):
     rng = held(v, bits).amax(-1, keepdim=True)[:, :, 1:2] - held(v, bits).amin(-1, keepdim=True)[:, :, 1:2]
     assert ((o.double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -21 * rng).all()
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -18 * want_lse).all()  # 16 products of 2^-23, a few roundings of 2^-24, of scores that do not cancel
+
+
+def test_lse_of_one_position():
+    """The score itself, to 2^-22 of it and of 1: sums of at most 64 products with 14 bits in all, a few of the last ones dropped."""
+    d, B = 64, 512
+    g = torch.Generator("cuda").manual_seed(120)
+    q = torch.randint(-3, 4, (B, 1, 1, d), generator=g, device="cuda").half()
+    k = torch.randint(0, 16, (B, 1, 1, d), generator=g, device="cuda").half()  # zero 0 and scale 1 where 0 and 15 occur
+    k[..., 0], k[..., 1] = 0, 15
+    table, pages = tables(g, B, 1)
+    cache = QuantizedKVCache(pages, 1, d, bits=4, page_size=16)
+    kv_cache_write(cache, k, k, table, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    one = torch.ones(B, dtype=torch.int32, device="cuda")
+    _, lse = kv_cache_attn(q, cache, table, one, None, False, 2.0 ** -6, True)
+    want = (q.double() * k.double()).sum(-1) * 2.0 ** -6
+    assert ((lse.double() - want).abs() <= 2.0 ** -21 * (1 + want.abs())).all(), (lse.double() - want).abs().max().item()
