@@ -1,4 +1,4 @@
-// The packed form of a quantised KV cache: what kv_write.cuh writes, kv_read.cuh reads back and kv_attn.cuh attends over.
+// The packed form of a quantised KV cache: what kv_write.cuh writes and reads back and kv_attn.cuh attends over.
 //
 // A position of a head holds d values of K and d of V. Each of the two is kept as d whole numbers n of BITS (4 or 8) bits and two
 // 16-bit numbers, scale and zero, of the cache's type: value = zero + scale n, with

@@ -4,7 +4,7 @@
     cache = QuantizedKVCache(num_pages, heads, head_dim, bits=4, page_size=64, dtype=torch.float16, device="cuda")
     kv_cache_write(cache, k, v, page_table, start, count=None)          # positions start[b] + i, i < count[b]
     o = kv_cache_attn(q, cache, page_table, lengths, device_type, causal=False, softmax_scale=None, return_lse=False)
-    k, v = kv_cache_read(cache, page_table, start, count, length)       # dense again, for flash_attn_func
+    k, v = kv_cache_read(cache, page_table, start, count, length)       # dense again, for flash_attn_func over equal lengths
 
 A position of a head of K or V is held as whole numbers n of 4 or 8 bits with a scale and a zero of the cache's type and stands for
 ``zero + scale * n``: zero is the smallest of the head_dim values, scale their range over 2^bits - 1 rounded to the type, n the
@@ -126,7 +126,9 @@ def kv_cache_write(cache, k, v, page_table, start, count=None):
 
 def kv_cache_read(cache, page_table, start=None, count=None, length=None):
     """K and V [B, heads, length, head_dim] of positions start[b] + i (from 0 without ``start``), rounded to the cache's dtype; rows
-    i >= count[b] are zeros. What flash_attn_func takes, when a prompt goes on behind what the cache holds."""
+    i >= count[b] are zeros. For a prompt that goes on behind what the cache holds by more than 64 positions: flash_attn_func takes them
+    with each head repeated for the heads of q that share it. It has no lengths and would attend to the zeros, so sequences of
+    different lengths go through it one at a time (``page_table[b:b + 1]``, ``length`` of that sequence)."""
     op = "kv_cache_read"
     if not isinstance(length, int) or isinstance(length, bool) or not 0 < length <= 1 << 30:
         _fail(f"{op}: length must be a positive integer, got {length!r}")
@@ -143,7 +145,8 @@ def kv_cache_attn(q, cache, page_table, lengths, device_type=None, causal=False,
     """flash_attn_func over the first lengths[b] positions of each sequence, for up to 64 queries: q [B, Hq, Lq, head_dim], Hq a
     multiple of the cache's heads (query heads h Hq/heads ... share head h). With ``causal`` the queries are the last Lq positions:
     query i sees j <= i + lengths[b] - Lq. A query that sees nothing gets 0 (lse -inf). ``softmax_scale=None`` is 0.125, as there.
-    The values zero + scale * n are used as they are, without a rounding to 16 bits."""
+    The values zero + scale * n are used as they are, without a rounding to 16 bits. Up to 4096 sequences. ``device_type`` stands where
+    flash_attn_func has it and is not used: there is no tile configuration to look up."""
     scale = 0.125 if softmax_scale is None else softmax_scale
     if isinstance(cache, QuantizedKVCache):
         out = kv_ops().kv_attn(cache.data, *cache._form, page_table, lengths, q, scale, causal, return_lse)
@@ -155,7 +158,8 @@ def kv_cache_attn(q, cache, page_table, lengths, device_type=None, causal=False,
     if q.shape[1] % cache.heads != 0:
         _fail(f"{op}: q has {q.shape[1]} heads, not a multiple of the cache's {cache.heads}")
     if q.shape[2] > MAX_QUERIES:
-        _fail(f"{op}: {q.shape[2]} queries of a sequence, at most {MAX_QUERIES} (longer prompts: kv_cache_read and flash_attn_func)")
+        _fail(f"{op}: {q.shape[2]} queries of a sequence, at most {MAX_QUERIES} (longer prompts: kv_cache_read and "
+              "flash_attn_func, for sequences of one length)")
     if lengths is None:
         _fail(f"{op}: lengths must be a tensor")
     _check_per_sequence(op, page_table, lengths=lengths)

@@ -7,6 +7,8 @@ import torch
 from test_gpu_kv_cache import DT, FORMS, attention64, check_attn, held, i32, tables
 
 from attention_autotuner_b200 import _lib
+from attention_autotuner_b200.arch import B200
+from attention_autotuner_b200.ops.attention_interface import flash_attn_func
 from attention_autotuner_b200.ops.cache_interface import QuantizedKVCache, kv_cache_attn, kv_cache_read, kv_cache_write
 
 pytestmark = pytest.mark.gpu
@@ -248,3 +250,26 @@ def test_lse_of_one_position():
     _, lse = kv_cache_attn(q, cache, table, one, None, False, 2.0 ** -6, True)
     want = (q.double() * k.double()).sum(-1) * 2.0 ** -6
     assert ((lse.double() - want).abs() <= 2.0 ** -21 * (1 + want.abs())).all(), (lse.double() - want).abs().max().item()
+
+
+def test_a_ragged_prompt_goes_on_sequence_by_sequence():
+    """70 more positions behind 40 and 100, by flash_attn_func over what is read back of each. Probabilities and values rounded to
+    bf16, as in the test of equal lengths."""
+    B, H, group, d, new, scale = 2, 2, 4, 128, 70, 128 ** -0.5
+    lens = [40, 100]
+    g = torch.Generator("cuda").manual_seed(130)
+    k, v = (torch.randn(B, H, 170, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(B, H * group, new, d, generator=g, device="cuda").bfloat16()
+    table, pages = tables(g, B, 6)
+    cache = QuantizedKVCache(pages, H, d, bits=8, page_size=32, dtype=torch.bfloat16)
+    kv_cache_write(cache, k, v, table, i32(0, 0), i32(*lens))
+    more = [torch.stack([x[b, :, n:n + new] for b, n in enumerate(lens)]) for x in (k, v)]
+    kv_cache_write(cache, *more, table, i32(*lens))
+    with pytest.raises(ValueError, match="of one length"):
+        kv_cache_attn(q, cache, table, i32(*lens) + new, None, True, scale)
+    for b, n in enumerate(lens):
+        dk, dv = kv_cache_read(cache, table[b:b + 1], length=n + new)
+        o = flash_attn_func(q[b:b + 1], dk.repeat_interleave(group, 1), dv.repeat_interleave(group, 1), B200(), True, scale)
+        at = slice(b, b + 1), slice(None), slice(0, n + new)
+        want, _, weight = attention64(q[b:b + 1], held(k[at], 8), held(v[at], 8), i32(n + new), True, scale)
+        assert ((o.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2 * 2.0 ** -8 * weight[..., :-1]).all()
