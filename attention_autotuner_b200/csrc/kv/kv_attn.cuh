@@ -6,7 +6,7 @@
 //
 // What bounds it: reading the cache once, 136 bytes per position and head of K and V at 4 bits and d = 128. At the copy bandwidth
 // (6.55 TB/s) an SM takes in a block of 16 positions every 94 cycles, in which its four schedulers issue 376 instructions; a block
-// costs a warp about 245 (40 to unpack K, 64 to transpose and unpack V, 16 products, 50 for the softmax, the rest to fetch). So:
+// costs a warp about 279 (72 to unpack K, 64 to transpose and unpack V, 16 products, 50 for the softmax, the rest to fetch). So:
 //   * every warp works alone, on units of 16 or 32 positions that it fetches itself, 16 bytes a lane at a time, into a ring of its
 //     own: no warp waits for another until the last unit of a head is done;
 //   * S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 with positions, then channels, as the 16 rows: eight query rows fill the
@@ -30,14 +30,15 @@
 // as much as rounding the output to fp16, and turns one output in a few hundred to the other side of a rounding to bf16. Up to four rows
 // the second piece costs no product; beyond, it takes two bf16 rows of eight heads from 22.5 to 24.1 us, four from 32.9 to 37.5.
 //
-// Measured (B200, us, calls one after another; at the copy bandwidth): 8 sequences of 131072 positions, 32 heads over 8, d = 128, 4 bits,
-// fp16 200 (174), 5.7 TB/s; 2 of 16384, 16 heads, 8 bits, bf16 28.4 (21); 32 of up to 8192, 32 over 8, 4 bits, bf16 22.5 (10.8); 16 of
-// up to 4096, four queries, 8 bits, fp16 15.0 (3.1); one of 50001, 8 heads over one, d = 256 14.4 (2.0); 2 of 512, 4 heads, d = 64 6.5.
+// Measured (B200, us of the device, calls one after another in a captured graph; at the copy bandwidth): 8 sequences of 131072 positions, 32
+// heads over 8, d = 128, 4 bits, fp16 210 (174), 5.4 TB/s, in bursts of a few ms, and 232 to 248 when the power limit sets the clock; 2 of
+// 16384, 16 heads, 8 bits, bf16 28.4 (21); 32 of up to 8192, 32 over 8, 4 bits, bf16 23.6 (10.8); 16 of up to 4096, four queries, 8 bits,
+// fp16 15.2 (3.1); one of 50001, 8 heads over one, d = 256 14.9 (2.0); 2 of 512, 4 heads, d = 64 6.8.
 // What is left of the short ones: 3 us until the first unit has come (lengths, table, unit: three trips to memory behind one
 // another), 1 us to add the warps' results, 3 us for the second kernel; of the middle ones as well that SMs with the same share
-// of the bytes finish up to 25% apart. Tried and not kept: units by bulk copies and mbarriers (one lane's work holds up its warp:
-// 214 -> 220), three units in the ring (the SMs finish further apart, 28.6 -> 30.2 for 8 bits), four CTAs per SM (spills, 227),
-// CTAs of one or two warps (the partial results of more runs: 22.2 -> 24.4, 23.2), twice the runs (28.5 -> 35.2).
+// of the bytes finish up to 25% apart. Tried and not kept, each against the kernel of its time: units by bulk copies and mbarriers (one
+// lane's work holds up its warp: 214 -> 220), three units in the ring (the SMs finish further apart, 28.6 -> 30.2 for 8 bits), four CTAs
+// per SM (spills, 227), CTAs of one or two warps (the partial results of more runs: 22.2 -> 24.4, 23.2), twice the runs (28.5 -> 35.2).
 #pragma once
 
 #include "../fast_div.cuh"
@@ -69,7 +70,7 @@ struct KvAttnConfig {
   // Units of a warp until its accumulators are added to fp32 sums in shared memory and begin anew. The tensor cores drop the bits that
   // do not fit, always the same way. A channel of V 40 above the others, which puts those at one end of their numbers, 65536 positions
   // in one CTA, fp16: up to 4.6e-4 of sum p |v| beyond the rounding of the output, after 1024 positions 6.1e-5, after 512 3.5e-5;
-  // 8 of 131072 take 202, 205 and 208 us.
+  // 8 of 131072 take 208, 210 and 213 us.
   static constexpr int HELD = 1024 / UNIT;
   static constexpr int RING_BYTES = NWARPS * NSTAGE * UNIT_BYTES;
   static constexpr int PART_STRIDE = D + 4;  // floats of a row: the rows of a warp's store fall on other banks
@@ -99,8 +100,8 @@ struct KvAttnParams {
 
 // Work: sequence b has n = units(b) of Cfg::UNIT positions for each (head, row block), and a head costs kKvHeadCost units more
 // (queries in, partial results out). The CTAs' runs are equal shares of that cost. Measured with 4 / 8 / 12 / 16 / 24 units: 64 sequences
-// of 100 to 4000 positions, 8 heads, d = 128, 4 bits 26.6 / 24.2 / 23.7 / 24.0 / 25.7 us (units of 32 positions); 32 of 64 to 4096,
-// four queries, 8 bits 34.3 / 30.3 / 26.6 / 24.6 / 25.2 (units of 16).
+// of 100 to 4000 positions, 8 heads, d = 128, 4 bits 27.8 / 25.2 / 24.3 / 24.9 / 26.7 us (units of 32 positions); 32 of 64 to 4096,
+// four queries, 8 bits 35.7 / 31.7 / 27.4 / 25.7 / 25.7 (units of 16).
 template <int UNIT>
 constexpr int kKvHeadCost = UNIT == 32 ? 12 : 16;
 // a / b for quotients far below 2^22: the product with the reciprocal is off by less than one.

@@ -147,10 +147,10 @@ int kv_attn_grid(int rows) {
 
 // Heads of few positions are not split, which saves the second kernel: a quarter of a head's units, one after another, then
 // take less than the parts' way through memory. With tables of 128 / 256 / 512 / 768 positions, a call split and whole, us:
-//   2 x 4 heads, d = 64, 4 bits   5.2  4.3 |  5.8  5.1 |  6.7  6.4 |  6.7  7.7
-//   16 x 8 heads, d = 128, 4 bits 6.1  5.6 |  8.3  7.4 |  9.4 10.3 | 10.6 13.0
-//   64 x 8 heads, d = 128, 4 bits 11.0 9.4 | 13.5 12.1 | 17.3 17.5 | 20.5 22.6
-//   8 x 8 heads, d = 128, 8 bits  6.2  5.6 |  7.4  6.9 |  8.5 10.4 |  8.9 13.5
+//   2 x 4 heads, d = 64, 4 bits   5.1  4.4 |  6.2  5.1 |  6.4  6.2 |  6.4  7.3
+//   16 x 8 heads, d = 128, 4 bits 6.6  6.1 |  8.1  7.5 |  9.5 10.0 | 11.0 12.7
+//   64 x 8 heads, d = 128, 4 bits 11.0 9.6 | 13.3 12.1 | 16.8 17.2 | 20.2 22.1
+//   8 x 8 heads, d = 128, 8 bits  5.8  5.4 |  7.4  6.9 |  8.4  9.4 |  8.9 12.0
 bool kv_attn_whole(long long positions, int d) { return positions * d <= 512 * 64; }
 
 template <class Cfg>

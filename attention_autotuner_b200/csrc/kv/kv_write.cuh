@@ -10,7 +10,7 @@
 // written, 17 for each read. Hence packed fp32 arithmetic for the numbers (kv_quantise) and the packed fma of the type for the values
 // (kv_values8).
 //
-// Measured (B200, us; at the copy bandwidth): 16 heads x 16384 positions, d = 128, 8 bits, bf16 written 38 (31; the ALUs are 62% busy, a
+// Measured (B200, us of the device; at the copy bandwidth): 16 heads x 16384 positions, d = 128, 8 bits, bf16 written 38 (31; the ALUs are 62% busy, a
 // bf16 row needs its largest numbers put right), read 32 (31); 4 x 16 heads of up to 2999, 4 bits, bf16 read 19.1 (16.3); 64 x 8 heads,
 // one position each, written and read 5.0. With a quotient for every number next to a half, where bf16 has one in 200: 78 written.
 #pragma once
