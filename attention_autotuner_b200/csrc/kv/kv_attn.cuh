@@ -409,15 +409,17 @@ __device__ __forceinline__ void kv_attn_blocks(KvAttnState<Cfg>& st, const uint8
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const int i = 2 * r + c;
-            if (EDGE && hidden[nb][nt][i]) continue;
-            top = fmaxf(top, y[nb][nt][i]);
-            wide = fmaxf(wide, y[nb][nt][i] + __log2f(vs[nb][r]));
-          }
+          for (int r = 0; r < R; ++r)
+            if (!EDGE || !hidden[nb][nt][2 * r + c]) top = fmaxf(top, y[nb][nt][2 * r + c]);
         // The reference is a whole number, so that what it moves by is taken out of the sums exactly.
         const float mn = fmaxf(st.m[nt][c], ceilf(kv_max_rows<Cfg::HALF>(top)));
-        wide = kv_max_rows<Cfg::HALF>(wide) - mn;  // of the largest weight
+        // of the largest weight; a logarithm added to a score would be lost where a step of fp32 is above it
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (!EDGE || !hidden[nb][nt][2 * r + c]) wide = fmaxf(wide, y[nb][nt][2 * r + c] - mn + __log2f(vs[nb][r]));
+        wide = kv_max_rows<Cfg::HALF>(wide);
         const int drop = static_cast<int>(fminf(mn - st.m[nt][c], 252.f));  // 252 from -inf too, and where nothing was seen yet
         const float f = kv_fall(mn - st.m[nt][c]);
         st.m[nt][c] = mn;

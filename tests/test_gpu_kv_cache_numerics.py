@@ -209,17 +209,20 @@ def test_tables_that_could_hold_more_than_the_kernels_count():
     assert _lib.kv_status() == 3
 
 
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 12, 2.0 ** 100])
 @pytest.mark.parametrize("group", [1, 8, 16])
 @pytest.mark.parametrize("name", ["fp16", "bf16"])
 @pytest.mark.parametrize("bits", [4, 8])
-def test_scores_of_any_size(bits, name, group):
+def test_scores_of_any_size(bits, name, group, size):
     """Scores up to 1e10, where a step of fp32 is 1000: the largest takes all, and the output is its value, rounded."""
+    if name == "fp16" and size > 2.0 ** 13:
+        size = 1 / 4096
     dtype, d, B = DT[name], 128, 100
     g = torch.Generator("cuda").manual_seed(110)
     sign = torch.where(torch.rand(B, 1, 1, d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
     q = 6e4 * sign * (0.5 + 0.5 * torch.rand(B, group, 1, d, generator=g, device="cuda"))
     k = 6e4 * sign * torch.tensor([0.2, 1.0, 0.5, -1.0], device="cuda")[:, None] * (0.9 + 0.1 * torch.rand(B, 1, 4, d, generator=g, device="cuda"))
-    v = torch.randn(B, 1, 4, d, generator=g, device="cuda")
+    v = torch.randn(B, 1, 4, d, generator=g, device="cuda") * size
     q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
     table, pages = tables(g, B, 1)
     cache = QuantizedKVCache(pages, 1, d, bits=bits, page_size=16, dtype=dtype)
@@ -232,7 +235,8 @@ def test_scores_of_any_size(bits, name, group):
     assert torch.equal(want, hv)
     # the value is put together of scale n and zero, each with a rounding of fp32 (the scale in pieces of 2^-22)
     rng = held(v, bits).amax(-1, keepdim=True)[:, :, 1:2] - held(v, bits).amin(-1, keepdim=True)[:, :, 1:2]
-    assert ((o.double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -21 * rng).all()
+    half = torch.finfo(dtype).eps / 2 * want.abs().clamp(min=torch.finfo(dtype).smallest_normal)
+    assert ((o.double() - want).abs() <= half + 2.0 ** -21 * rng).all()
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -18 * want_lse).all()  # 16 products of 2^-23, a few roundings of 2^-24, of scores that do not cancel
 
 
@@ -273,3 +277,29 @@ def test_a_ragged_prompt_goes_on_sequence_by_sequence():
         at = slice(b, b + 1), slice(None), slice(0, n + new)
         want, _, weight = attention64(q[b:b + 1], held(k[at], 8), held(v[at], 8), i32(n + new), True, scale)
         assert ((o.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2 * 2.0 ** -8 * weight[..., :-1]).all()
+
+
+@pytest.mark.parametrize("group,Lq", [(1, 1), (2, 2), (3, 2), (4, 4)])
+@pytest.mark.parametrize("bits,d,name", FORMS)
+def test_sums_of_long_shares(bits, d, name, group, Lq):
+    """Heads that each lie in a CTA or two, so that a warp goes over several times 1024 positions, with references that rise, values
+    whose scales change from position to position, NaN in hidden places, and lengths that end anywhere."""
+    dtype, B, L = DT[name], 700, 20000
+    g = torch.Generator("cuda").manual_seed(140)
+    k, v = (torch.randn(1, 1, L, d, generator=g, device="cuda") for _ in range(2))
+    k *= torch.linspace(0.05, 1.5, L, device="cuda")[:, None]
+    v *= torch.exp2(torch.randint(-6, 7, (L, 1), generator=g, device="cuda").float())
+    k, v = k.to(dtype), v.to(dtype)
+    v[:, :, -1] = math.nan
+    cache, table = one_sequence(k, v, bits, 64, g)
+    q = torch.randn(B, group, Lq, d, generator=g, device="cuda").to(dtype)
+    lengths = torch.randint(0, L, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[:3] = i32(L - 1, L - 1024, 4096)
+    o, lse = kv_cache_attn(q, cache, table.expand(B, -1), lengths, None, True, d ** -0.5, True)
+    assert o.isfinite().all()
+    hk, hv = held(k, bits), held(v[:, :, :-1], bits)
+    for b in (0, 1, 2, 350, 699):
+        n = int(lengths[b])
+        at = slice(b, b + 1)
+        want = attention64(q[at], hk[:, :, :n], hv[:, :, :n], lengths[at], True, d ** -0.5)
+        check_attn(o[at], lse[at], *want)
